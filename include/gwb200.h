@@ -310,6 +310,58 @@ int gwb_awq_qweight_unpack(const void* qweight, int64_t N, int64_t K, void* weig
 int gwb_awq_w4a16_mm(const void* x, const void* weight, const void* wscales, const void* wzeros,
                      const void* bias, int64_t M, int64_t N, int64_t K, void* out, void* stream);
 
+/* ---- Transformer-block operators beside the quantised linears: layer norm
+ * with modulation, rotary positions. No counterpart in the reference's own
+ * code, which leaves them to its model library. `dtype` codes:
+ * GWB_DTYPE_F32 / _BF16 / _F16. Strides are in elements; pointers and strides
+ * need only the element's alignment (16-byte ones run faster). */
+enum { GWB_DTYPE_F32 = 0, GWB_DTYPE_BF16 = 1, GWB_DTYPE_F16 = 2 };
+
+/* y [M, D] = ((x - mean) * rstd * weight + bias) * (1 + scale) + shift, per
+ * row of x [M, D] (row stride x_stride), rstd = 1 / sqrt(var + eps), f32
+ * statistics. weight / bias [D] and scale / shift [M / rows_per_mod, D]
+ * (sample strides scale_stride / shift_stride, 0 = one row for all) may each
+ * be NULL; *_f32 != 0: that pair is f32, else of x's type. mean / rstd
+ * f32 [M] (for the backward pass) are both written or both NULL. */
+int gwb_layer_norm(const void* x, int64_t x_stride, const void* weight, const void* bias,
+                   int affine_f32, const void* scale, int64_t scale_stride, const void* shift,
+                   int64_t shift_stride, int mod_f32, int64_t M, int64_t D,
+                   int64_t rows_per_mod, float eps, int dtype, void* y, float* mean, float* rstd,
+                   void* stream);
+
+/* f32 elements of the scratch `work` that gwb_layer_norm_backward needs when
+ * any parameter gradient is asked for (0 when none of the sizes is positive). */
+int64_t gwb_layer_norm_backward_work(int64_t M, int64_t D, int64_t rows_per_mod);
+
+/* Gradients of gwb_layer_norm: dx [M, D], dweight / dbias [D] (in the affine
+ * pair's type), dscale / dshift [M / rows_per_mod, D] (in the modulation
+ * pair's type), each NULL when not wanted. Column sums are f32, joined in a
+ * fixed order without atomics: the same call gives the same bits. */
+int gwb_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                            const float* mean, const float* rstd, const void* weight,
+                            const void* bias, int affine_f32, const void* scale,
+                            int64_t scale_stride, int mod_f32, int64_t M, int64_t D,
+                            int64_t rows_per_mod, int dtype, void* dx, void* dweight, void* dbias,
+                            void* dscale, void* dshift, float* work, void* stream);
+
+/* Rotary positions of q [B, S, q_heads, head_dim] and k [B, S, k_heads,
+ * head_dim] (k_heads 0: no keys; strides {batch, token, head}, the last
+ * dimension dense): pairs of the first 2 * n features turn by
+ * positions[b, s, axis[i]] * inv_freq[i] and are multiplied by `scale`;
+ * pair i is (2 i, 2 i + 1) when interleaved, else (i, n + i). The remaining
+ * features are copied; with x == out (in place) they are left alone.
+ * inverse != 0 turns by the negative angle (the backward pass). positions:
+ * position_kind 0 int64, 1 int32, 2 f32, strides {batch, token, axis};
+ * inv_freq f64 [n]; axis int32 [n] with values below `axes`, or NULL for
+ * axis 0. Angles are reduced in f64. */
+int gwb_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+               int64_t q_heads, const void* k, const int64_t* k_strides, void* k_out,
+               const int64_t* k_out_strides, int64_t k_heads, const void* positions,
+               int position_kind, const int64_t* position_strides, const double* inv_freq,
+               const int32_t* axis, int64_t axes, int64_t B, int64_t S, int64_t n,
+               int64_t head_dim, float scale, int interleaved, int inverse, int dtype,
+               void* stream);
+
 /* Reads and clears the device-side error flag set by a bounded wait that
  * expired (0 = none; 1 TMA producer, 2 MMA thread, 3 epilogue, 4 unpack
  * warps, 5 the INT4 quantiser's x boxes). Synchronises the device. */

@@ -24,7 +24,9 @@ HERE = Path(__file__).resolve().parent
 PKG = HERE.parent / "gen_worker_b200"
 OUT = PKG / "_lib" / "libgwb200.so"
 TORCH_OUT = PKG / "_lib" / "libgwb200_torch.so"
-SOURCES = ["capi.cu", "act_quant.cu", "gemm.cu", "codec.cu", "awq.cu", "noalloc.cu", "gwb.h", "ptx.cuh"]
+SOURCES = ["capi.cu", "act_quant.cu", "gemm.cu", "codec.cu", "awq.cu", "norm.cu", "rotary.cu",
+           "noalloc.cu", "gwb.h", "ptx.cuh", "elem.cuh"]
+TORCH_SOURCES = ["torch_ext.cpp", "torch_block.cpp"]
 HEADER = HERE.parent.parent / "include" / "gwb200.h"
 
 NVCC_FLAGS = [
@@ -68,13 +70,13 @@ def torch_ext_stale() -> bool:
     if not TORCH_OUT.exists():
         return True
     t = TORCH_OUT.stat().st_mtime
-    deps = [HERE / "torch_ext.cpp", HEADER, Path(__file__), OUT]
+    deps = [*(HERE / f for f in TORCH_SOURCES), HEADER, Path(__file__), OUT]
     return any(d.stat().st_mtime > t for d in deps if d.exists())
 
 
 def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
-    """libgwb200_torch.so: the TORCH_LIBRARY(cozy_kernels) face of the C ABI,
-    compiled with g++ against this interpreter's torch and linked to
+    """libgwb200_torch.so: the TORCH_LIBRARY(cozy_kernels) face of the C ABI and
+    the block operators with their autograd (torch.ops.gwb200), compiled with g++ against this interpreter's torch and linked to
     libgwb200.so beside it (rpath $ORIGIN)."""
     if not force and not torch_ext_stale():
         return TORCH_OUT
@@ -85,7 +87,7 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
     tmp = TORCH_OUT.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            *[f"-I{p}" for p in ce.include_paths()], f"-I{cuda_inc}",
-           str(HERE / "torch_ext.cpp"), "-o", str(tmp),
+           *[str(HERE / f) for f in TORCH_SOURCES], "-o", str(tmp),
            *[f"-L{p}" for p in ce.library_paths()], "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch", f"-L{OUT.parent}", "-l:libgwb200.so", "-Wl,-rpath,$ORIGIN"]
     if verbose:

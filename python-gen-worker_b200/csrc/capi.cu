@@ -9,6 +9,8 @@
 #include "gemm.cu"
 #include "codec.cu"
 #include "awq.cu"
+#include "norm.cu"
+#include "rotary.cu"
 #include "../../include/gwb200.h"
 
 #ifndef GWB_ARCH_STRING
@@ -60,6 +62,8 @@ inline int check_w4a4_shape(int64_t M, int64_t N, int64_t K, int rank_pad) {
   if (rank_pad < 0 || rank_pad > 128 || rank_pad % 16) return GWB_E_SHAPE;
   return GWB_SUCCESS;
 }
+
+inline bool known_dtype(int d) { return d == GWB_F32 || d == GWB_BF16 || d == GWB_F16; }
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -385,6 +389,95 @@ int gwb_awq_w4a16_mm(const void* x, const void* weight, const void* wscales, con
       static_cast<const __nv_bfloat16*>(bias), static_cast<__nv_bfloat16*>(out), (int)M, (int)N,
       (int)K, S(stream));
   return e == cudaSuccess ? GWB_SUCCESS : GWB_E_LAUNCH;
+}
+
+static_assert(GWB_DTYPE_F32 == (int)GWB_F32 && GWB_DTYPE_BF16 == (int)GWB_BF16 &&
+              GWB_DTYPE_F16 == (int)GWB_F16, "dtype codes");
+
+int gwb_layer_norm(const void* x, int64_t x_stride, const void* weight, const void* bias,
+                   int affine_f32, const void* scale, int64_t scale_stride, const void* shift,
+                   int64_t shift_stride, int mod_f32, int64_t M, int64_t D,
+                   int64_t rows_per_mod, float eps, int dtype, void* y, float* mean, float* rstd,
+                   void* stream) {
+  if (M == 0) return GWB_SUCCESS;
+  if (!fits_int(M) || !fits_int(D) || D == 0 || rows_per_mod <= 0 || M % rows_per_mod)
+    return GWB_E_SHAPE;
+  if (!known_dtype(dtype) || !x || !y || (mean == nullptr) != (rstd == nullptr))
+    return GWB_E_SHAPE;
+  gwb::norm::FwdArgs a{x, x_stride, {weight, affine_f32 != 0, 0}, {bias, affine_f32 != 0, 0},
+                       {scale, mod_f32 != 0, scale_stride}, {shift, mod_f32 != 0, shift_stride},
+                       y, mean, rstd, M, (int)D, rows_per_mod, eps};
+  return gwb::launch_layer_norm(a, dtype, S(stream));
+}
+
+int64_t gwb_layer_norm_backward_work(int64_t M, int64_t D, int64_t rows_per_mod) {
+  if (M <= 0 || D <= 0 || rows_per_mod <= 0) return 0;
+  const int64_t samples = M / rows_per_mod;
+  return samples * gwb::norm::chunks_of(samples, rows_per_mod) * 2 * D;
+}
+
+int gwb_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                            const float* mean, const float* rstd, const void* weight,
+                            const void* bias, int affine_f32, const void* scale,
+                            int64_t scale_stride, int mod_f32, int64_t M, int64_t D,
+                            int64_t rows_per_mod, int dtype, void* dx, void* dweight, void* dbias,
+                            void* dscale, void* dshift, float* work, void* stream) {
+  if (!fits_int(M) || !fits_int(D) || D == 0 || rows_per_mod < 0 || !known_dtype(dtype))
+    return GWB_E_SHAPE;
+  const bool sums = dweight || dbias || dscale || dshift;
+  if (M == 0) {
+    // no rows: the parameters' gradients are zero
+    const size_t wide = affine_f32 || dtype == GWB_F32 ? 4 : 2;
+    if (dweight && cudaMemsetAsync(dweight, 0, (size_t)D * wide, S(stream)) != cudaSuccess)
+      return GWB_E_LAUNCH;
+    if (dbias && cudaMemsetAsync(dbias, 0, (size_t)D * wide, S(stream)) != cudaSuccess)
+      return GWB_E_LAUNCH;
+    return GWB_SUCCESS;
+  }
+  if (rows_per_mod == 0 || M % rows_per_mod) return GWB_E_SHAPE;
+  if (!dy || !x || !mean || !rstd || (sums && !work)) return GWB_E_SHAPE;
+  if (!dx && !sums) return GWB_SUCCESS;
+  const int64_t samples = M / rows_per_mod;
+  const int chunks = gwb::norm::chunks_of(samples, rows_per_mod);
+  if (samples * chunks > 0x7fffffff) return GWB_E_CAPACITY;
+  const int64_t chunk_rows = (rows_per_mod + chunks - 1) / chunks;
+  gwb::norm::Param w{weight, affine_f32 != 0, 0}, b{bias, affine_f32 != 0, 0},
+      s{scale, mod_f32 != 0, scale_stride};
+  gwb::norm::BwdArgs a{dy, dy_stride, x, x_stride, mean, rstd, w, b, s, dx,
+                       sums ? work : nullptr, rows_per_mod, (int)D, chunks, chunk_rows};
+  gwb::norm::SumArgs t{work, samples, chunks, (int)D, w, b, s, dweight, dbias, dscale, dshift};
+  return gwb::launch_layer_norm_backward(a, samples, t, sums, dtype, S(stream));
+}
+
+int gwb_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+               int64_t q_heads, const void* k, const int64_t* k_strides, void* k_out,
+               const int64_t* k_out_strides, int64_t k_heads, const void* positions,
+               int position_kind, const int64_t* position_strides, const double* inv_freq,
+               const int32_t* axis, int64_t axes, int64_t B, int64_t S_, int64_t n,
+               int64_t head_dim, float scale, int interleaved, int inverse, int dtype,
+               void* stream) {
+  if (B < 0 || S_ < 0 || q_heads < 0 || k_heads < 0) return GWB_E_SHAPE;
+  if (B == 0 || S_ == 0 || q_heads + k_heads == 0) return GWB_SUCCESS;
+  if (!fits_int(B * S_) || !fits_int(S_) || !fits_int(B) || q_heads + k_heads > (1 << 20))
+    return GWB_E_SHAPE;
+  if (n < 0 || head_dim < 1 || head_dim > 4096 || 2 * n > head_dim || axes < 1 || axes > 64 ||
+      position_kind < 0 || position_kind > 2 || !known_dtype(dtype))
+    return GWB_E_SHAPE;
+  if (q_heads && (!q || !q_out || !q_strides || !q_out_strides)) return GWB_E_SHAPE;
+  if (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) return GWB_E_SHAPE;
+  if (!positions || !position_strides || (n && !inv_freq)) return GWB_E_SHAPE;
+  const bool in_place = (!q_heads || q == q_out) && (!k_heads || k == k_out);
+  if (in_place && n == 0) return GWB_SUCCESS;
+  const auto heads = [](const void* x, const int64_t* xs, void* y, const int64_t* ys, int64_t h) {
+    if (h == 0) return gwb::rotary::Heads{};
+    return gwb::rotary::Heads{x, y, xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], (int)h};
+  };
+  gwb::rotary::Args a{heads(q, q_strides, q_out, q_out_strides, q_heads),
+                      heads(k, k_strides, k_out, k_out_strides, k_heads), positions,
+                      position_kind, position_strides[0], position_strides[1],
+                      position_strides[2], inv_freq, axis, (int)axes, B * S_, (int)S_, (int)n,
+                      (int)head_dim, scale, inverse != 0, in_place, 1, 1};
+  return gwb::launch_rotary(a, interleaved != 0, dtype, S(stream));
 }
 
 int gwb_set_wait_limit(long long cycles) {

@@ -16,6 +16,9 @@ enum GwbStatus : int {
   GWB_E_CAPACITY = 8,   // request exceeds a fixed capacity
 };
 
+// Element types of the block operators (GWB_DTYPE_* of the C ABI).
+enum GwbDtype : int { GWB_F32 = 0, GWB_BF16 = 1, GWB_F16 = 2 };
+
 namespace gwb {
 int launch_act_int4(const void* x, const void* smooth, const void* down_t, void* codes,
                     void* ascale, void* la, int M, int K, int rank_pad, bool mma_form,

@@ -12,7 +12,9 @@ from .modules import (LAYOUT_INT4, LAYOUT_NVFP4, Fp8RowwiseLinear, SvdqInt4Linea
                       build_svdq_int4_linear, build_svdq_nvfp4_linear, build_w8a8_int8_linear,
                       fp8_rowwise_from_linear, quantize_fp8_rows, quantize_int4_rows,
                       quantize_int8_rows, svdq_int4_from_linear, swap_linears)
-from . import awq, codec, ops
+from .norm import ModulatedLayerNorm, layer_norm, norm_from_layer_norm
+from .rope import RotaryEmbedding, rotary, rotary_, rotary_frequencies
+from . import awq, codec, norm, ops, rope
 
 __all__ = [
     "LAYOUT_INT4", "LAYOUT_NVFP4", "NativeKernelError", "Fp8RowwiseLinear", "SvdqInt4Linear",
@@ -20,5 +22,7 @@ __all__ = [
     "build_svdq_int4_linear", "build_svdq_nvfp4_linear", "build_w8a8_int8_linear",
     "device_error", "fp8_rowwise_from_linear", "quantize_fp8_rows",
     "extension_available", "extension_reason", "library_path", "ops", "awq", "codec",
+    "ModulatedLayerNorm", "RotaryEmbedding", "layer_norm", "norm", "norm_from_layer_norm", "rope",
+    "rotary", "rotary_", "rotary_frequencies",
     "quantize_int4_rows", "quantize_int8_rows", "svdq_int4_from_linear", "swap_linears",
 ]

@@ -24,7 +24,8 @@ c_void_p = ctypes.c_void_p
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 
-# (name, argtypes); every entry point returns int status.
+# (name, argtypes); every entry point returns int status, but for the sizes in
+# _RETURNS_I64 and the status text.
 _SIGNATURES = {
     "gwb_build_info": [ctypes.c_char_p, ctypes.c_size_t],
     "gwb_probe_add_one": [c_void_p, c_void_p, c_i64, c_void_p],
@@ -72,6 +73,18 @@ _SIGNATURES = {
     "gwb_awq_qweight_unpack": [c_void_p, c_i64, c_i64, c_void_p],
     "gwb_awq_w4a16_mm": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64,
                          c_void_p, c_void_p],
+    "gwb_layer_norm": [c_void_p, c_i64, c_void_p, c_void_p, c_int, c_void_p, c_i64, c_void_p, c_i64,
+                       c_int, c_i64, c_i64, c_i64, ctypes.c_float, c_int, c_void_p, c_void_p,
+                       c_void_p, c_void_p],
+    "gwb_layer_norm_backward_work": [c_i64, c_i64, c_i64],
+    "gwb_layer_norm_backward": [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_int, c_void_p, c_i64, c_int, c_i64, c_i64, c_i64,
+                                c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_void_p],
+    "gwb_rotary": [c_void_p, ctypes.POINTER(c_i64), c_void_p, ctypes.POINTER(c_i64), c_i64,
+                   c_void_p, ctypes.POINTER(c_i64), c_void_p, ctypes.POINTER(c_i64), c_i64,
+                   c_void_p, c_int, ctypes.POINTER(c_i64), c_void_p, c_void_p, c_i64, c_i64, c_i64,
+                   c_i64, c_i64, ctypes.c_float, c_int, c_int, c_int, c_void_p],
     "gwb_fp8_gemm": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64,
                      c_int, c_void_p, c_void_p],
     "gwb_fp8_linear": [c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64, c_int,
@@ -87,6 +100,7 @@ _SIGNATURES = {
     "gwb_status_string": [c_int],
 }
 
+_RETURNS_I64 = {"gwb_layer_norm_backward_work"}
 EXPORTED = tuple(_SIGNATURES)
 
 
@@ -114,7 +128,8 @@ def lib() -> ctypes.CDLL:
     for name, argtypes in _SIGNATURES.items():
         fn = getattr(handle, name)
         fn.argtypes = argtypes
-        fn.restype = ctypes.c_char_p if name == "gwb_status_string" else c_int
+        fn.restype = (ctypes.c_char_p if name == "gwb_status_string" else
+                      c_i64 if name in _RETURNS_I64 else c_int)
     return handle
 
 
@@ -201,3 +216,24 @@ def require() -> ctypes.CDLL:
     if reason is not None:
         raise NativeKernelError(f"gwb200 native path unavailable: {reason}")
     return lib()
+
+
+_BLOCK_READY: set = set()
+
+
+def block_ops(x):
+    """``torch.ops.gwb200`` with the block operators (layer norm, rotary,
+    gated linear) of ``libgwb200_torch.so`` loaded, once the device of ``x``
+    has passed :func:`require`. The first call on a device probes it with a
+    launch and a synchronise: make it before any stream capture."""
+    import torch
+
+    if x.device.index not in _BLOCK_READY:
+        torch_ops()
+        from . import _fakes  # noqa: F401 — the operators' shapes for torch.compile
+        if isinstance(x, torch._subclasses.FakeTensor):
+            return torch.ops.gwb200
+        with torch.cuda.device(x.device):
+            require()
+        _BLOCK_READY.add(x.device.index)
+    return torch.ops.gwb200
