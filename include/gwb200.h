@@ -311,7 +311,7 @@ int gwb_awq_w4a16_mm(const void* x, const void* weight, const void* wscales, con
                      const void* bias, int64_t M, int64_t N, int64_t K, void* out, void* stream);
 
 /* ---- Transformer-block operators beside the quantised linears: layer norm
- * with modulation, rotary positions. No counterpart in the reference's own
+ * with modulation, rotary positions, gated feed-forward projections. No counterpart in the reference's own
  * code, which leaves them to its model library. `dtype` codes:
  * GWB_DTYPE_F32 / _BF16 / _F16. Strides are in elements; pointers and strides
  * need only the element's alignment (16-byte ones run faster). */
@@ -361,6 +361,32 @@ int gwb_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64
                const int32_t* axis, int64_t axes, int64_t B, int64_t S, int64_t n,
                int64_t head_dim, float scale, int interleaved, int inverse, int dtype,
                void* stream);
+
+/* Gated feed-forward projections, bf16 or f16 (`dtype` GWB_DTYPE_BF16 /
+ * _F16): h [M, F] = act(x w_gate^T + b_gate) * (x w_up^T + b_up), one kernel.
+ * x [M, D] (row stride x_stride), w_gate / w_up [F, D] contiguous, biases [F]
+ * or NULL; `activation` GWB_ACT_*. f32 accumulation, one rounding. D % 8 == 0,
+ * F % 8 == 0, strides % 8 == 0, 16-byte aligned pointers. M == 0 is a no-op. */
+enum { GWB_ACT_SILU = 0, GWB_ACT_GELU = 1, GWB_ACT_GELU_TANH = 2 };
+
+int gwb_gated_linear(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
+                     const void* b_gate, const void* b_up, int64_t M, int64_t D, int64_t F,
+                     int activation, int dtype, void* h, void* stream);
+
+/* Bytes of the 256-byte aligned scratch `work` of gwb_gated_linear_backward
+ * (0 when a size is not positive). */
+int64_t gwb_gated_linear_backward_work(int64_t M, int64_t F);
+
+/* Gradients of gwb_gated_linear, each NULL when not wanted: dx [M, D],
+ * dw_gate / dw_up [F, D], db_gate / db_up [F], from dh [M, F] (row stride
+ * dh_stride). The projections are computed again rather than kept from the
+ * forward call; dg and du are rounded to `dtype` as the operands of the
+ * gradients' products. No atomics: the same call gives the same bits. */
+int gwb_gated_linear_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
+                              const void* w_gate, const void* w_up, const void* b_gate,
+                              const void* b_up, int64_t M, int64_t D, int64_t F, int activation,
+                              int dtype, void* dx, void* dw_gate, void* dw_up, void* db_gate,
+                              void* db_up, void* work, void* stream);
 
 /* Reads and clears the device-side error flag set by a bounded wait that
  * expired (0 = none; 1 TMA producer, 2 MMA thread, 3 epilogue, 4 unpack

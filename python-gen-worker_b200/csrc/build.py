@@ -25,7 +25,7 @@ PKG = HERE.parent / "gen_worker_b200"
 OUT = PKG / "_lib" / "libgwb200.so"
 TORCH_OUT = PKG / "_lib" / "libgwb200_torch.so"
 SOURCES = ["capi.cu", "act_quant.cu", "gemm.cu", "codec.cu", "awq.cu", "norm.cu", "rotary.cu",
-           "noalloc.cu", "gwb.h", "ptx.cuh", "elem.cuh"]
+           "gated.cu", "noalloc.cu", "gwb.h", "ptx.cuh", "elem.cuh"]
 TORCH_SOURCES = ["torch_ext.cpp", "torch_block.cpp"]
 HEADER = HERE.parent.parent / "include" / "gwb200.h"
 

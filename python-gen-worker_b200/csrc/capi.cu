@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <cstdio>
 #include <cstring>
+#include "../../include/gwb200.h"
 #include "gwb.h"
 #include "ptx.cuh"
 #include "act_quant.cu"
@@ -11,6 +12,7 @@
 #include "awq.cu"
 #include "norm.cu"
 #include "rotary.cu"
+#include "gated.cu"
 #include "../../include/gwb200.h"
 
 #ifndef GWB_ARCH_STRING
@@ -478,6 +480,61 @@ int gwb_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64
                       position_strides[2], inv_freq, axis, (int)axes, B * S_, (int)S_, (int)n,
                       (int)head_dim, scale, inverse != 0, in_place, 1, 1};
   return gwb::launch_rotary(a, interleaved != 0, dtype, S(stream));
+}
+
+static int gated_sizes(int64_t M, int64_t D, int64_t F, int activation, int dtype) {
+  if (!fits_int(M) || !fits_int(D) || !fits_int(F) || D == 0 || F == 0 || D % 8 || F % 8)
+    return GWB_E_SHAPE;
+  // tile counts are 32-bit
+  if ((M / 128 + 1) * (F / 128 + 1) > 0x7fffffff || (F / 64 + 2) * (D / 256 + 1) > 0x7fffffff)
+    return GWB_E_CAPACITY;
+  if (activation < GWB_ACT_SILU || activation > GWB_ACT_GELU_TANH) return GWB_E_SHAPE;
+  return dtype == GWB_BF16 || dtype == GWB_F16 ? GWB_SUCCESS : GWB_E_SHAPE;
+}
+
+int gwb_gated_linear(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
+                     const void* b_gate, const void* b_up, int64_t M, int64_t D, int64_t F,
+                     int activation, int dtype, void* h, void* stream) {
+  if (int rc = gated_sizes(M, D, F, activation, dtype)) return rc;
+  if (M == 0) return GWB_SUCCESS;
+  if (!x || !w_gate || !w_up || !h) return GWB_E_SHAPE;
+  if (x_stride < D || x_stride % 8) return GWB_E_SHAPE;
+  if (!al16(x) || !al16(w_gate) || !al16(w_up) || !al16(h) || (b_gate && !al16(b_gate)) ||
+      (b_up && !al16(b_up)))
+    return GWB_E_ALIGN;
+  return gwb::launch_gated_forward(x, x_stride, w_gate, w_up, b_gate, b_up, (int)M, (int)D, (int)F,
+                                   activation, dtype, h, S(stream));
+}
+
+int64_t gwb_gated_linear_backward_work(int64_t M, int64_t F) {
+  if (!fits_int(M) || !fits_int(F) || M == 0 || F == 0) return 0;
+  return gwb::gated_backward_work((int)M, (int)F);
+}
+
+int gwb_gated_linear_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
+                              const void* w_gate, const void* w_up, const void* b_gate,
+                              const void* b_up, int64_t M, int64_t D, int64_t F, int activation,
+                              int dtype, void* dx, void* dw_gate, void* dw_up, void* db_gate,
+                              void* db_up, void* work, void* stream) {
+  if (int rc = gated_sizes(M, D, F, activation, dtype)) return rc;
+  if (M == 0) {
+    // no rows: the parameters' gradients are zero
+    void* const grads[4] = {dw_gate, dw_up, db_gate, db_up};
+    for (int i = 0; i < 4; ++i)
+      if (grads[i] && cudaMemsetAsync(grads[i], 0, (size_t)F * (i < 2 ? D : 1) * 2, S(stream)) !=
+                          cudaSuccess)
+        return GWB_E_LAUNCH;
+    return GWB_SUCCESS;
+  }
+  if (!dh || !x || !w_gate || !w_up || !work) return GWB_E_SHAPE;
+  if (x_stride < D || x_stride % 8 || dh_stride < F || dh_stride % 8) return GWB_E_SHAPE;
+  for (const void* p : {dh, x, w_gate, w_up, b_gate, b_up, (const void*)dx, (const void*)dw_gate,
+                        (const void*)dw_up, (const void*)work})
+    if (!al16(p)) return GWB_E_ALIGN;
+  if (!dx && !dw_gate && !dw_up && !db_gate && !db_up) return GWB_SUCCESS;
+  gwb::GatedBackward w{dh, dh_stride, x, x_stride, w_gate, w_up, b_gate, b_up, (int)M, (int)D,
+                       (int)F, activation, dx, dw_gate, dw_up, db_gate, db_up, work};
+  return gwb::launch_gated_backward(w, dtype, S(stream));
 }
 
 int gwb_set_wait_limit(long long cycles) {

@@ -1,0 +1,492 @@
+// Gated feed-forward projections, bf16 or f16, forward and backward:
+//
+//   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) * u        [M, F]
+//   dg = dh * u * act'(g),  du = dh * act(g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  db = column sums
+//
+// x [M, D], Wg and Wu [F, D]. Tensor cores bound all of it (4 M D F operations
+// forward, 8 M D F backward) except at few rows, where reading the weights
+// does. One persistent TMA-fed tcgen05 kernel serves the four products; the
+// operands' majorness is a template argument, so no operand is transposed in
+// memory: the backward products read W, x and dg / du as they lie, through
+// MN-major shared-memory descriptors.
+//
+//   FORWARD  128 x (128 gate | 128 up) tile: both projections accumulate side
+//            by side in TMEM, so activation and product happen in registers
+//            and g and u never reach memory.
+//   DGATE    the same tile again; the epilogue reads dh and writes dg and du
+//            (rounded to the operand type: they are tensor-core operands next).
+//   DX       dg Wg + du Wu as one chain of K = 2 F into one accumulator.
+//   DW       dg^T x and du^T x, K = M.
+//
+// Accumulators, activations and column sums are f32; every output is rounded
+// once.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <atomic>
+#include "gwb.h"
+#include "ptx.cuh"
+#include "elem.cuh"
+
+namespace gwb {
+namespace gated {
+
+enum Mode { FORWARD, DGATE, DX, DW };
+
+constexpr int BM = 128, BN = 256, BK = 64;      // BK elements = one 128-byte swizzle row
+constexpr int STAGES = 4;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int MN_BOX = 64 * BK * 2;             // a 64 (MN) x 64 (K) box of an MN-major operand
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int THREADS = 384, EPI0 = 4, EPI_WARPS = 8;
+constexpr int NACC = 2, TMEM_COLS = NACC * BN;
+// Tiles are walked in groups of 16 row tiles: 148 tiles at once then read
+// about 16 row tiles and 9 column tiles (twice as wide), the least operand
+// bytes for a product of the two counts.
+constexpr int GROUP = 16;
+
+struct Args {
+  const void* bg; const void* bu;     // FORWARD, DGATE: biases [F] or null
+  const void* dh; int64_t dhs;        // DGATE: [M, F], row stride
+  void* o0; void* o1;                 // h | dg, du | dx | dWg, dWu
+  int M, D, F, act;
+  int tiles_m, tiles_n, half0, ntiles;
+};
+
+// ------------------------------------------------------------- activations
+struct ActValue { float act, slope; };
+
+// act(g), and act'(g) when SLOPE. silu and the tanh form of GELU are
+// g * sigmoid(t): 1 - sigmoid is taken without cancellation on either side.
+template <bool SLOPE>
+__device__ __forceinline__ ActValue activation(float g, int kind) {
+  ActValue r;
+  r.slope = 0.0f;
+  if (kind == GWB_ACT_GELU) {
+    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    r.act = g * cdf;
+    if (SLOPE) r.slope = cdf + g * (0.39894228040143268f * __expf(-0.5f * g * g));
+    return r;
+  }
+  constexpr float c = 2.0f * 0.79788456080286536f, k = 0.044715f;   // 2 sqrt(2 / pi)
+  const float t = kind == GWB_ACT_SILU ? g : c * (g + k * g * g * g);
+  const float e = __expf(-t);
+  const float s = __fdividef(1.0f, 1.0f + e);
+  r.act = g * s;
+  if (SLOPE) {
+    const float q = t >= 0.0f ? e * s : 1.0f - s;                   // 1 - s
+    const float dt = kind == GWB_ACT_SILU ? 1.0f : c * (1.0f + 3.0f * k * g * g);
+    r.slope = s + g * (s * q) * dt;
+  }
+  return r;
+}
+
+// ------------------------------------------------------------- descriptors
+// MN-major operand, 128-byte swizzle: 64 MN elements are one 128-byte row,
+// eight K rows a 1024-byte atom (SBO, to the next eight K), the next 64 MN
+// elements `lbo` bytes on.
+__device__ __forceinline__ uint64_t sdesc_mn128(uint32_t saddr, uint32_t lbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) |
+         ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <typename T, bool A_MN, bool B_MN>
+__host__ __device__ constexpr uint32_t idesc16() {
+  constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
+         ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+
+struct Tile { int m0, n0, half; };
+
+template <int MODE>
+__device__ __forceinline__ Tile tile_of(const Args& a, int t) {
+  const int per = GROUP * a.tiles_n, first = t / per * GROUP;
+  const int rows = min(a.tiles_m - first, GROUP), in = t % per;
+  const int tm = first + in % rows, tn = in / rows;
+  if (MODE == DW) {
+    const int tf = (a.F + BM - 1) / BM;
+    return {(tm % tf) * BM, tn * BN, a.half0 + tm / tf};
+  }
+  return {tm * BM, tn * (MODE == DX ? BN : BN / 2), 0};
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void load8(const T* p, float (&f)[N]) {
+  Pack<T, 8> v;
+  v.load(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = v.get(j);
+}
+
+template <int MODE, typename T>
+__global__ void __launch_bounds__(THREADS, 1)
+gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
+             const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1,
+             const Args a) {
+  constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + NACC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + NACC);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kext = MODE == DX ? a.F : MODE == DW ? a.M : a.D;
+  const int nk1 = (kext + BK - 1) / BK;               // k-blocks of one segment
+  const int nk = MODE == DX ? 2 * nk1 : nk1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < NACC; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], EPI_WARPS); }
+    fence_barrier_init();
+    tma_prefetch_desc(&tA0);
+    tma_prefetch_desc(&tB0);
+    if (MODE != DW) tma_prefetch_desc(&tB1);
+    if (B_MN) tma_prefetch_desc(&tA1);
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // register hand-off as in the W8A8 kernel: 384 x 168 at launch, the first
+  // warpgroup down to 40, the two epilogue warpgroups up to 232
+  if (warp < EPI0) {
+    regs_dec<40>();
+    if (warp == 0 && lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < a.ntiles; tile += gridDim.x) {
+        const Tile t = tile_of<MODE>(a, tile);
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, GWB_ERR_TIMEOUT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + s * STAGE_BYTES;
+          uint8_t* sb = sa + A_BYTES;
+          mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
+          if constexpr (MODE == FORWARD || MODE == DGATE) {
+            tma_load_2d(sa, &tA0, &full[s], kb * BK, t.m0);
+            tma_load_2d(sb, &tB0, &full[s], kb * BK, t.n0);
+            tma_load_2d(sb + B_BYTES / 2, &tB1, &full[s], kb * BK, t.n0);
+          } else if constexpr (MODE == DX) {
+            const bool up = kb >= nk1;
+            const int k0 = (kb - (up ? nk1 : 0)) * BK;
+            tma_load_2d(sa, up ? &tA1 : &tA0, &full[s], k0, t.m0);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j)
+              tma_load_2d(sb + j * MN_BOX, up ? &tB1 : &tB0, &full[s], t.n0 + 64 * j, k0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j)
+              tma_load_2d(sa + j * MN_BOX, t.half ? &tA1 : &tA0, &full[s], t.m0 + 64 * j, kb * BK);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j)
+              tma_load_2d(sb + j * MN_BOX, &tB0, &full[s], t.n0 + 64 * j, kb * BK);
+          }
+        }
+      }
+    } else if (warp == 1 && lane == 0) {
+      constexpr uint32_t idesc = idesc16<T, A_MN, B_MN>();
+      int it = 0, lt = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < a.ntiles; tile += gridDim.x, ++lt) {
+        const int b = lt & 1;
+        if (!mbar_wait(&acc_empty[b], ((lt >> 1) & 1) ^ 1, GWB_ERR_TIMEOUT_MMA)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + b * BN;
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&full[s], (it / STAGES) & 1, GWB_ERR_TIMEOUT_MMA)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t ab = smem_u32(smem + s * STAGE_BYTES), bb = ab + A_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            mma_f16(d, A_MN ? sdesc_mn128(ab + 2048 * k, MN_BOX) : sdesc_k128(ab + 32 * k),
+                    B_MN ? sdesc_mn128(bb + 2048 * k, MN_BOX) : sdesc_k128(bb + 32 * k), idesc,
+                    (kb > 0 || k > 0) ? 1u : 0u);
+          mma_commit(&empty[s]);
+        }
+        if (ok) mma_commit(&acc_full[b]);
+      }
+    }
+  } else {
+    regs_inc<232>();
+    const int q = warp & 3, side = (warp - EPI0) >> 2;
+    int lt = 0;
+    for (int tile = blockIdx.x; tile < a.ntiles; tile += gridDim.x, ++lt) {
+      const Tile t = tile_of<MODE>(a, tile);
+      const int b = lt & 1;
+      if (!mbar_wait(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
+      __syncwarp();
+      tc_fence_after();
+      uint32_t v[128];
+      const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + b * BN;
+      const int row = t.m0 + 32 * q + lane;
+      if constexpr (MODE == FORWARD || MODE == DGATE) {
+        // v[0..63] gate and v[64..127] up of columns n0 + 64 side ..
+        tmem_ld32(base + 64 * side, v);
+        tmem_ld32(base + 64 * side + 32, v + 32);
+        tmem_ld32(base + 128 + 64 * side, v + 64);
+        tmem_ld32(base + 160 + 64 * side, v + 96);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32(base + 128 * side + c, v + c);
+      }
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[b]);
+      if constexpr (MODE == FORWARD || MODE == DGATE) {
+        if (row >= a.M) continue;
+        const int n0 = t.n0 + 64 * side;
+#pragma unroll
+        for (int c = 0; c < 64; c += 8) {
+          if (n0 + c >= a.F) break;
+          float g[8], u[8], p[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            g[j] = __uint_as_float(v[c + j]);
+            u[j] = __uint_as_float(v[64 + c + j]);
+          }
+          if (a.bg) {
+            load8(static_cast<const T*>(a.bg) + n0 + c, p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] += p[j];
+          }
+          if (a.bu) {
+            load8(static_cast<const T*>(a.bu) + n0 + c, p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] += p[j];
+          }
+          const size_t at = (size_t)row * a.F + n0 + c;
+          Pack<T, 8> o0, o1;
+          if constexpr (MODE == FORWARD) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o0.set(j, activation<false>(g[j], a.act).act * u[j]);
+            o0.store(static_cast<T*>(a.o0) + at);
+          } else {
+            load8(static_cast<const T*>(a.dh) + (size_t)row * a.dhs + n0 + c, p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const ActValue f = activation<true>(g[j], a.act);
+              o0.set(j, p[j] * u[j] * f.slope);
+              o1.set(j, p[j] * f.act);
+            }
+            o0.store(static_cast<T*>(a.o0) + at);
+            o1.store(static_cast<T*>(a.o1) + at);
+          }
+        }
+      } else {
+        if (row >= (MODE == DX ? a.M : a.F)) continue;
+        T* out = static_cast<T*>(t.half ? a.o1 : a.o0) + (size_t)row * a.D;
+        const int n0 = t.n0 + 128 * side;
+#pragma unroll
+        for (int c = 0; c < 128; c += 8) {
+          if (n0 + c >= a.D) break;
+          Pack<T, 8> o;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o.set(j, __uint_as_float(v[c + j]));
+          o.store(out + n0 + c);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// ------------------------------------------------------------- bias gradients
+// Column sums of dg (blockIdx.z 0) and du (1): 256 columns a CTA (eight a
+// lane), its warps taking rows of one chunk in turn; partials [2][chunks][F],
+// joined in a fixed order by column_join_kernel.
+template <typename T>
+__global__ void __launch_bounds__(256)
+column_sums_kernel(const T* __restrict__ dg, const T* __restrict__ du, int M, int F,
+                   int chunk_rows, float* __restrict__ partial) {
+  __shared__ float acc[8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = blockIdx.x * 256 + lane * 8;
+  const T* src = blockIdx.z ? du : dg;
+  const int r0 = blockIdx.y * chunk_rows, r1 = min(M, r0 + chunk_rows);
+  float s[8] = {};
+  if (c0 < F)
+    for (int r = r0 + warp; r < r1; r += 8) {
+      float p[8];
+      load8(src + (size_t)r * F + c0, p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += p[j];
+    }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[warp][lane * 8 + j] = s[j];
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < F) {
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += acc[w][threadIdx.x];
+    partial[((size_t)blockIdx.z * gridDim.y + blockIdx.y) * F + c] = t;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+column_join_kernel(const float* __restrict__ partial, int chunks, int F, T* dbg, T* dbu) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  T* out = blockIdx.y ? dbu : dbg;
+  if (c >= F || out == nullptr) return;
+  float t = 0.0f;
+  for (int k = 0; k < chunks; ++k) t += partial[((size_t)blockIdx.y * chunks + k) * F + c];
+  out[c] = from_f32<T>(t);
+}
+
+// ------------------------------------------------------------- host
+// 2-D tensor of 16-bit elements, rows `ld` elements apart, box {64, by}
+inline int tmap16(CUtensorMap* m, const void* base, bool bf16, int64_t cols, int64_t rows,
+                  int64_t ld, int by) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return GWB_E_DRIVER;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)by}, es[2] = {1, 1};
+  const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        2, const_cast<void*>(base), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? GWB_SUCCESS : GWB_E_TMAP;
+}
+
+template <int MODE, typename T>
+int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0,
+           const CUtensorMap& b1, Args a, cudaStream_t st) {
+  auto kern = gated_kernel<MODE, T>;
+  // the shared-memory limit is a property of the function on each device
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return GWB_E_LAUNCH;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) !=
+        cudaSuccess)
+      return GWB_E_LAUNCH;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const int n_sm = sm_count();
+  kern<<<a.ntiles < n_sm ? a.ntiles : n_sm, THREADS, SMEM_BYTES, st>>>(a0, a1, b0, b1, a);
+  return launch_status();
+}
+
+// Tensor maps are encoded by the driver, which wants a current context: a
+// thread that has made no runtime call yet (autograd's) has none until its
+// device is set.
+inline int bind_context() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return GWB_E_LAUNCH;
+  return GWB_SUCCESS;
+}
+
+inline int cdiv(int a, int b) { return (a + b - 1) / b; }
+
+template <typename T>
+int projections(bool dgate, const void* x, int64_t xs, const void* wg, const void* wu, Args a,
+                cudaStream_t st) {
+  constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+  if (int rc = bind_context()) return rc;
+  CUtensorMap tx, tg, tu;
+  if (int rc = tmap16(&tx, x, bf, a.D, a.M, xs, BM)) return rc;
+  if (int rc = tmap16(&tg, wg, bf, a.D, a.F, a.D, BN / 2)) return rc;
+  if (int rc = tmap16(&tu, wu, bf, a.D, a.F, a.D, BN / 2)) return rc;
+  a.tiles_m = cdiv(a.M, BM);
+  a.tiles_n = cdiv(a.F, BN / 2);
+  a.ntiles = a.tiles_m * a.tiles_n;
+  return dgate ? launch<DGATE, T>(tx, tx, tg, tu, a, st) : launch<FORWARD, T>(tx, tx, tg, tu, a, st);
+}
+
+// Chunks of rows of the bias gradient's column sums: about four CTAs a
+// multiprocessor, at least 32 rows each.
+inline int bias_chunks(int M, int F) {
+  const int tiles = cdiv(F, 256) * 2, want = cdiv(148 * 4, tiles), most = cdiv(M, 32);
+  return want < most ? (want > 0 ? want : 1) : (most > 0 ? most : 1);
+}
+
+template <typename T>
+int backward(const GatedBackward& w, cudaStream_t st) {
+  constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+  const int M = w.M, D = w.D, F = w.F;
+  uint8_t* p = static_cast<uint8_t*>(w.work);
+  const size_t plane = ((size_t)M * F * 2 + 255) / 256 * 256;
+  void* dg = p;
+  void* du = p + plane;
+  float* partial = reinterpret_cast<float*>(p + 2 * plane);
+  Args a{};
+  a.bg = w.bg; a.bu = w.bu; a.dh = w.dh; a.dhs = w.dhs; a.o0 = dg; a.o1 = du;
+  a.M = M; a.D = D; a.F = F; a.act = w.act;
+  if (int rc = projections<T>(true, w.x, w.xs, w.wg, w.wu, a, st)) return rc;
+  if (w.dx) {
+    CUtensorMap ag, au, bgm, bum;
+    if (int rc = tmap16(&ag, dg, bf, F, M, F, BM)) return rc;
+    if (int rc = tmap16(&au, du, bf, F, M, F, BM)) return rc;
+    if (int rc = tmap16(&bgm, w.wg, bf, D, F, D, BK)) return rc;
+    if (int rc = tmap16(&bum, w.wu, bf, D, F, D, BK)) return rc;
+    Args c = a;
+    c.o0 = w.dx;
+    c.tiles_m = cdiv(M, BM);
+    c.tiles_n = cdiv(D, BN);
+    c.ntiles = c.tiles_m * c.tiles_n;
+    if (int rc = launch<DX, T>(ag, au, bgm, bum, c, st)) return rc;
+  }
+  if (w.dwg || w.dwu) {
+    CUtensorMap ag, au, bx;
+    if (int rc = tmap16(&ag, dg, bf, F, M, F, BK)) return rc;
+    if (int rc = tmap16(&au, du, bf, F, M, F, BK)) return rc;
+    if (int rc = tmap16(&bx, w.x, bf, D, M, w.xs, BK)) return rc;
+    Args c = a;
+    c.o0 = w.dwg;
+    c.o1 = w.dwu;
+    c.half0 = w.dwg ? 0 : 1;
+    c.tiles_m = cdiv(F, BM) * (w.dwg && w.dwu ? 2 : 1);
+    c.tiles_n = cdiv(D, BN);
+    c.ntiles = c.tiles_m * c.tiles_n;
+    if (int rc = launch<DW, T>(ag, au, bx, bx, c, st)) return rc;
+  }
+  if (w.dbg || w.dbu) {
+    const int chunks = bias_chunks(M, F);
+    column_sums_kernel<T><<<dim3(cdiv(F, 256), chunks, 2), 256, 0, st>>>(
+        static_cast<const T*>(dg), static_cast<const T*>(du), M, F, cdiv(M, chunks), partial);
+    if (int rc = launch_status()) return rc;
+    column_join_kernel<T><<<dim3(cdiv(F, 256), 2), 256, 0, st>>>(
+        partial, chunks, F, static_cast<T*>(w.dbg), static_cast<T*>(w.dbu));
+    return launch_status();
+  }
+  return GWB_SUCCESS;
+}
+
+}  // namespace gated
+
+int64_t gated_backward_work(int M, int F) {
+  const int64_t plane = ((int64_t)M * F * 2 + 255) / 256 * 256;
+  return 2 * plane + (int64_t)2 * gated::bias_chunks(M, F) * F * 4;
+}
+
+int launch_gated_forward(const void* x, int64_t xs, const void* wg, const void* wu, const void* bg,
+                         const void* bu, int M, int D, int F, int act, int dtype, void* h,
+                         cudaStream_t st) {
+  gated::Args a{};
+  a.bg = bg; a.bu = bu; a.o0 = h; a.M = M; a.D = D; a.F = F; a.act = act;
+  return dtype == GWB_BF16 ? gated::projections<__nv_bfloat16>(false, x, xs, wg, wu, a, st)
+                           : gated::projections<__half>(false, x, xs, wg, wu, a, st);
+}
+
+int launch_gated_backward(const GatedBackward& w, int dtype, cudaStream_t st) {
+  return dtype == GWB_BF16 ? gated::backward<__nv_bfloat16>(w, st)
+                           : gated::backward<__half>(w, st);
+}
+
+}  // namespace gwb

@@ -20,6 +20,14 @@ enum GwbStatus : int {
 enum GwbDtype : int { GWB_F32 = 0, GWB_BF16 = 1, GWB_F16 = 2 };
 
 namespace gwb {
+struct GatedBackward {
+  const void* dh; int64_t dhs;     // [M, F], row stride
+  const void* x; int64_t xs;       // [M, D], row stride
+  const void* wg; const void* wu; const void* bg; const void* bu;
+  int M, D, F, act;
+  void* dx; void* dwg; void* dwu; void* dbg; void* dbu;   // any may be null
+  void* work;
+};
 int launch_act_int4(const void* x, const void* smooth, const void* down_t, void* codes,
                     void* ascale, void* la, int M, int K, int rank_pad, bool mma_form,
                     cudaStream_t st);

@@ -1,5 +1,5 @@
-// torch.ops.gwb200: layer norm with modulation and rotary positions over the
-// C ABI (include/gwb200.h), with their gradients.
+// torch.ops.gwb200: layer norm with modulation, rotary positions and gated
+// feed-forward projections over the C ABI (include/gwb200.h), with their gradients.
 //
 // The dispatcher's CUDA key holds the plain calls; the Autograd key records a
 // node only when a gradient is wanted and otherwise goes straight below, so
@@ -502,6 +502,138 @@ void rotary_inplace_autograd(Tensor q, const OptTensor& k, const Tensor& positio
   if (has(k)) torch::autograd::increment_version(*k);
 }
 
+// ---------------------------------------------------------------- gated projections
+bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0; }
+
+// Rows at one stride that TMA can read (16-byte steps), else a copy.
+Tensor tma_rows_of(const Tensor& x, int64_t* stride) {
+  const int64_t d = x.size(-1);
+  if (row_stride_of(x, stride) && *stride >= d && *stride % 8 == 0 && aligned16(x)) return x;
+  *stride = d;
+  if (x.is_contiguous() && aligned16(x)) return x;
+  // contiguous() of a dense but misaligned view would return the view itself
+  return at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)).copy_(x);
+}
+
+struct GatedShape { int64_t rows, d, f; int dtype; };
+
+GatedShape gated_shape(const Tensor& x, const Tensor& wg, const Tensor& wu, const OptTensor& bg,
+                       const OptTensor& bu, int64_t act) {
+  NEED(x.is_cuda(), "x must be a CUDA tensor (no CPU path), got ", x.device());
+  NEED(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
+       "x must be bfloat16 or float16, got ", x.scalar_type());
+  NEED(x.dim() >= 1, "x must be [..., D]");
+  GatedShape g{0, x.size(-1), wg.dim() == 2 ? wg.size(0) : 0, dtype_code(x, "x")};
+  NEED(g.d >= 8 && g.d % 8 == 0, "x has ", g.d, " features; a positive multiple of 8 is needed");
+  g.rows = x.numel() / g.d;
+  const auto weight = [&](const Tensor& w, const char* name) {
+    need_on(w, name, x);
+    NEED(w.scalar_type() == x.scalar_type(), name, " must be ", x.scalar_type(), ", got ",
+         w.scalar_type());
+    NEED(w.dim() == 2 && w.size(0) == g.f && w.size(1) == g.d, name, " must be [", g.f, ", ", g.d,
+         "], got ", w.sizes());
+    NEED(w.is_contiguous() && aligned16(w), name, " must be contiguous and 16-byte aligned");
+  };
+  weight(wg, "w_gate");
+  weight(wu, "w_up");
+  NEED(g.f >= 8 && g.f % 8 == 0, "w_gate has ", g.f, " rows; a positive multiple of 8 is needed");
+  const auto bias = [&](const OptTensor& b, const char* name) {
+    if (!has(b)) return;
+    need_on(*b, name, x);
+    NEED(b->scalar_type() == x.scalar_type() && b->dim() == 1 && b->size(0) == g.f, name,
+         " must be ", x.scalar_type(), " [", g.f, "], got ", b->scalar_type(), " ", b->sizes());
+    NEED(b->is_contiguous() && aligned16(*b), name, " must be contiguous and 16-byte aligned");
+  };
+  bias(bg, "b_gate");
+  bias(bu, "b_up");
+  NEED(act >= GWB_ACT_SILU && act <= GWB_ACT_GELU_TANH, "unknown activation code ", act);
+  return g;
+}
+
+Tensor gated_linear_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu, const OptTensor& bg,
+                         const OptTensor& bu, int64_t act) {
+  const GatedShape g = gated_shape(x, wg, wu, bg, bu, act);
+  const c10::cuda::CUDAGuard guard(x.device());
+  int64_t xs = 0;
+  const Tensor xr = tma_rows_of(x, &xs);
+  auto shape = x.sizes().vec();
+  shape.back() = g.f;
+  Tensor h = at::empty(shape, x.options().memory_format(at::MemoryFormat::Contiguous));
+  check_status(gwb_gated_linear(xr.const_data_ptr(), xs, wg.const_data_ptr(), wu.const_data_ptr(),
+                                ptr(bg), ptr(bu), g.rows, g.d, g.f, (int)act, g.dtype,
+                                h.data_ptr(), stream_of(x)),
+               "gated_linear");
+  return h;
+}
+
+// -> (dx, dw_gate, dw_up, db_gate, db_up); one not asked for is empty [0]
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward_cuda(
+    const Tensor& dh, const Tensor& x, const Tensor& wg, const Tensor& wu, const OptTensor& bg,
+    const OptTensor& bu, int64_t act, std::array<bool, 5> mask) {
+  const GatedShape g = gated_shape(x, wg, wu, bg, bu, act);
+  const c10::cuda::CUDAGuard guard(x.device());
+  need_on(dh, "dh", x);
+  NEED(dh.scalar_type() == x.scalar_type() && dh.dim() == x.dim() && dh.size(-1) == g.f &&
+           dh.sizes().slice(0, dh.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
+       "dh must be ", x.scalar_type(), " of x's shape with ", g.f, " features, got ", dh.sizes());
+  NEED((!mask[3] || has(bg)) && (!mask[4] || has(bu)),
+       "a gradient was asked for of a bias that is not given");
+  int64_t xs = 0, ds = 0;
+  const Tensor xr = tma_rows_of(x, &xs), dr = tma_rows_of(dh, &ds);
+  const auto out = [&](bool on, at::IntArrayRef shape) {
+    return at::empty(on ? shape : at::IntArrayRef{0},
+                     x.options().memory_format(at::MemoryFormat::Contiguous));
+  };
+  Tensor dx = out(mask[0], x.sizes()), dwg = out(mask[1], wg.sizes()), dwu = out(mask[2], wu.sizes());
+  Tensor dbg = out(mask[3], {g.f}), dbu = out(mask[4], {g.f});
+  Tensor work = at::empty({gwb_gated_linear_backward_work(g.rows, g.f)},
+                          x.options().dtype(at::kByte));
+  const auto at_ = [](bool on, Tensor& t) { return on ? t.data_ptr() : nullptr; };
+  check_status(gwb_gated_linear_backward(
+                   dr.const_data_ptr(), ds, xr.const_data_ptr(), xs, wg.const_data_ptr(),
+                   wu.const_data_ptr(), ptr(bg), ptr(bu), g.rows, g.d, g.f, (int)act, g.dtype,
+                   at_(mask[0], dx), at_(mask[1], dwg), at_(mask[2], dwu), at_(mask[3], dbg),
+                   at_(mask[4], dbu), work.data_ptr(), stream_of(x)),
+               "gated_linear_backward");
+  return {dx, dwg, dwu, dbg, dbu};
+}
+
+struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu,
+                        const OptTensor& bg, const OptTensor& bu, int64_t act) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = op_of<decltype(gated_linear_cuda)>("gwb200::gated_linear");
+    Tensor h = op.call(x, wg, wu, bg, bu, act);
+    ctx->save_for_backward({x, wg, wu, has(bg) ? *bg : Tensor(), has(bu) ? *bu : Tensor()});
+    ctx->saved_data["act"] = act;
+    return h;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    refuse_second_order("gated_linear_backward", grads[0], v[0], v[1], v[2], v[3], v[4]);
+    if (!grads[0].defined()) return variable_list(6);
+    std::array<bool, 5> mask{};
+    for (int i = 0, given = 0; i < 5; ++i)
+      if (v[i].defined()) mask[i] = ctx->needs_input_grad(given++);
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = op_of<decltype(gated_linear_backward_cuda)>("gwb200::gated_linear_backward");
+    auto [dx, dwg, dwu, dbg, dbu] = op.call(grads[0], v[0], v[1], v[2], opt(v[3]), opt(v[4]),
+                                            ctx->saved_data["act"].toInt(), mask);
+    const auto give = [&](int i, Tensor& t) { return mask[i] ? t : Tensor(); };
+    return {give(0, dx), give(1, dwg), give(2, dwu), give(3, dbg), give(4, dbu), Tensor()};
+  }
+};
+
+Tensor gated_linear_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu,
+                             const OptTensor& bg, const OptTensor& bu, int64_t act) {
+  if (at::GradMode::is_enabled() &&
+      (wants(x) || wants(wg) || wants(wu) || wants(bg) || wants(bu)))
+    return GatedLinearFn::apply(x, wg, wu, bg, bu, act);
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = op_of<decltype(gated_linear_cuda)>("gwb200::gated_linear");
+  return op.call(x, wg, wu, bg, bu, act);
+}
+
 }  // namespace gwb200_block
 
 TORCH_LIBRARY_FRAGMENT(gwb200, m) {
@@ -516,6 +648,10 @@ TORCH_LIBRARY_FRAGMENT(gwb200, m) {
         "bool interleaved, float scale, bool inverse) -> (Tensor, Tensor)");
   m.def("rotary_(Tensor(a!) q, Tensor(b!)? k, Tensor positions, Tensor inv_freq, Tensor? axis, "
         "bool interleaved, float scale, bool inverse) -> ()");
+  m.def("gated_linear(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, "
+        "int activation) -> Tensor");
+  m.def("gated_linear_backward(Tensor dh, Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, "
+        "Tensor? b_up, int activation, bool[5] mask) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(gwb200, CUDA, m) {
@@ -524,10 +660,13 @@ TORCH_LIBRARY_IMPL(gwb200, CUDA, m) {
   m.impl("layer_norm_backward", &gwb200_block::layer_norm_backward_cuda);
   m.impl("rotary", &gwb200_block::rotary_cuda);
   m.impl("rotary_", &gwb200_block::rotary_inplace_cuda);
+  m.impl("gated_linear", &gwb200_block::gated_linear_cuda);
+  m.impl("gated_linear_backward", &gwb200_block::gated_linear_backward_cuda);
 }
 
 TORCH_LIBRARY_IMPL(gwb200, Autograd, m) {
   m.impl("layer_norm", &gwb200_block::layer_norm_autograd);
   m.impl("rotary", &gwb200_block::rotary_autograd);
   m.impl("rotary_", &gwb200_block::rotary_inplace_autograd);
+  m.impl("gated_linear", &gwb200_block::gated_linear_autograd);
 }

@@ -33,3 +33,14 @@ def _(q, k, positions, inv_freq, axis, interleaved, scale, inverse):
 @torch.library.register_fake("gwb200::rotary_")
 def _(q, k, positions, inv_freq, axis, interleaved, scale, inverse):
     return None
+
+
+@torch.library.register_fake("gwb200::gated_linear")
+def _(x, w_gate, w_up, b_gate, b_up, activation):
+    return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
+
+
+@torch.library.register_fake("gwb200::gated_linear_backward")
+def _(dh, x, w_gate, w_up, b_gate, b_up, activation, mask):
+    given = (x, w_gate, w_up, b_gate, b_up)
+    return tuple(t.new_empty(t.shape) if on else x.new_empty(0) for t, on in zip(given, mask))

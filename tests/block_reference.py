@@ -97,3 +97,44 @@ def rotary64(x, positions, inv_freq, axis, interleaved, scale, sign=1.0):
 # (fraction of a turn to f32: pi), sincospi and the scale on each (3), two
 # products and a sum (3).
 ROTARY_COUNT = math.ceil(math.pi + 3 + 3)
+
+
+# ---------------------------------------------------------------- gated projections
+def gated64(x, wg, wu, bg, bu, activation):
+    """(h, g, u) in 64 bits."""
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    g, u = x @ wg.t(), x @ wu.t()
+    g = g if bg is None else g + bg.double()
+    u = u if bu is None else u + bu.double()
+    if activation == "silu":
+        a = g * torch.special.expit(g)
+    elif activation == "gelu":
+        a = g * torch.special.ndtr(g)
+    else:
+        a = 0.5 * g * (1 + torch.tanh(math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)))
+    return a * u, g, u
+
+
+def gated_magnitudes(x, wg, wu, bg, bu, dh, h64):
+    """f64 bounds of the errors that come before each output's own rounding.
+
+    A product's f32 accumulation over K terms is off by at most K * u times
+    the terms' magnitudes (any order). In units of u: e = K + 2 for g and u;
+    act and act' (slopes at most 1.13 and 1.7, act <= |g|) are off by 2 e
+    |g|'s magnitude + 16 (|g| + 1) of their own arithmetic (exp to 2 ulp of an
+    argument off by 3 roundings, at |t| <= 40 before it vanishes)."""
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    d = x.shape[1]
+    zero = torch.zeros(wg.shape[0], dtype=torch.float64)
+    bg, bu = (zero if b is None else b.double().abs() for b in (bg, bu))
+    gm, um = x.abs() @ wg.abs().t() + bg, x.abs() @ wu.abs().t() + bu
+    e = d + 2
+    g, u = h64[1].abs(), h64[2].abs()
+    act_err = (1.2 * e * gm + 48 * (g + 1)) * U
+    slope_err = (1.0 * e * gm + 96 * (g + 1)) * U
+    out = {"h": act_err * u + g * e * U * um + 4 * U * g * u}
+    if dh is not None:
+        dh = dh.double().abs()
+        out["dg"] = dh * (1.2 * e * U * um + u * slope_err + 4 * U * 1.2 * u)
+        out["du"] = dh * (act_err + 4 * U * g)
+    return out
