@@ -415,7 +415,7 @@ int gwb_layer_norm(const void* x, int64_t x_stride, const void* weight, const vo
 int64_t gwb_layer_norm_backward_work(int64_t M, int64_t D, int64_t rows_per_mod) {
   if (M <= 0 || D <= 0 || rows_per_mod <= 0) return 0;
   const int64_t samples = M / rows_per_mod;
-  return samples * gwb::norm::chunks_of(samples, rows_per_mod) * 2 * D;
+  return samples * gwb::norm::chunks_of(samples, rows_per_mod, D) * 2 * D;
 }
 
 int gwb_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
@@ -440,7 +440,7 @@ int gwb_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, in
   if (!dy || !x || !mean || !rstd || (sums && !work)) return GWB_E_SHAPE;
   if (!dx && !sums) return GWB_SUCCESS;
   const int64_t samples = M / rows_per_mod;
-  const int chunks = gwb::norm::chunks_of(samples, rows_per_mod);
+  const int chunks = gwb::norm::chunks_of(samples, rows_per_mod, D);
   if (samples * chunks > 0x7fffffff) return GWB_E_CAPACITY;
   const int64_t chunk_rows = (rows_per_mod + chunks - 1) / chunks;
   gwb::norm::Param w{weight, affine_f32 != 0, 0}, b{bias, affine_f32 != 0, 0},

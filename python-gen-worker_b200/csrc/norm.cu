@@ -17,7 +17,10 @@
 // backward. Column sums go through per-CTA partials and a second kernel in a
 // fixed order, without atomics, so gradients are the same on every run.
 #include <cuda_runtime.h>
+#include <algorithm>
+#include <initializer_list>
 #include "gwb.h"
+#include "ptx.cuh"
 #include "elem.cuh"
 
 namespace gwb {
@@ -84,16 +87,260 @@ __device__ __forceinline__ float block_sum(float v, float* slot) {
   return warp_sum(lane < nw ? slot[lane] : 0.0f);
 }
 
-// One row per warp (WARP, four rows per CTA) or per CTA; the row stays in
+// ------------------------------------------------ rows through shared memory
+// Bulk copies bring rows as the 16-byte granules that cover them, so a row may
+// start anywhere: `lead` bytes into its first granule. Nothing before the
+// granule of a row's first element or past the granule of its last is read,
+// and of the matrix's last granule only its elements.
+struct Span { const uint8_t* from; uint32_t lead, bytes; };
+
+template <typename T>
+__device__ __forceinline__ Span span_of(const T* first, int64_t n) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(first);
+  Span s;
+  s.lead = (uint32_t)(a & 15u);
+  s.from = reinterpret_cast<const uint8_t*>(a - s.lead);
+  s.bytes = (s.lead + (uint32_t)(n * sizeof(T)) + 15u) & ~15u;
+  return s;
+}
+
+// One thread: the copy of n elements at `first` to dst, to complete on `bar`
+// (whose expected bytes the caller has not announced yet); returns them.
+// `last`: nothing may be read behind the elements, so a part granule at the
+// end is stored by hand, ordered before the copy's completion by this
+// thread's own arrival.
+template <typename T>
+__device__ __forceinline__ uint32_t span_bytes(const T* first, int64_t n, bool last, uint8_t* dst) {
+  const Span s = span_of(first, n);
+  const uint32_t end = s.lead + (uint32_t)(n * sizeof(T));
+  if (!last || end == s.bytes) return s.bytes;
+  const uint32_t whole = end & ~15u;
+  for (uint32_t b = whole > s.lead ? whole : s.lead; b < end; b += sizeof(T))
+    *reinterpret_cast<T*>(dst + b) = *reinterpret_cast<const T*>(s.from + b);
+  return whole;
+}
+
+// After a wait that ran out: the copies in flight land (again with a limit)
+// before the shared memory goes to another CTA.
+__device__ __forceinline__ void drain(uint64_t* full, int stages, int from, int to) {
+  for (int k = from; k < to; ++k)
+    (void)mbar_wait(&full[k % stages], (k / stages) & 1, GWB_ERR_TIMEOUT_ACT);
+}
+
+// g = w (1 + s) and h = b (1 + s) + t of one sample's columns, f32, so that
+// y = z g + h
+template <typename T>
+__device__ __forceinline__ void combine(const Param& w, const Param& b, const Param& s,
+                                        const Param& t, int64_t smp, int c, float& g, float& h) {
+  float p[1], up = 1.0f;
+  if (s.p) { load_param<T, 1>(s, smp, c, p); up += p[0]; }
+  g = up;
+  h = 0.0f;
+  if (w.p) { load_param<T, 1>(w, 0, c, p); g *= p[0]; }
+  if (b.p) { load_param<T, 1>(b, 0, c, p); h = p[0] * up; }
+  if (t.p) { load_param<T, 1>(t, smp, c, p); h += p[0]; }
+}
+
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// f(i, column, column exists) for a lane's elements l, l + L, ...: eight at a
+// time without a test where all lanes have them (a test an element costs a
+// predicate that outlives the row's registers).
+template <int E, int LO, int L, typename F>
+__device__ __forceinline__ void each(int D, int l, const F& f) {
+#pragma unroll
+  for (int h = 0; h < E; h += 8) {
+    if (h + 8 <= LO || (h + 8) * L <= D) {
+#pragma unroll
+      for (int i = h; i < h + 8; ++i) f(i, l + i * L, true);
+    } else if (h * L < D) {
+#pragma unroll
+      for (int i = h; i < h + 8; ++i) f(i, l + i * L, l + i * L < D);
+    }
+  }
+}
+
+struct FwdPlan {
+  int chunks;                    // CTAs a sample
+  int64_t chunk_rows;            // rows of one, a multiple of slot_rows
+  int slot_rows, stages;         // rows a copy brings, slots a warp
+  uint32_t slot_bytes;
+};
+
+// A warp takes whole rows (32 / L at a time, L lanes each), E elements a
+// lane, from its own ring of bulk copies: no barrier but the one that shares
+// g and h, and few instructions a row besides the arithmetic, which a form
+// with a CTA per row spent on its reductions (21 us against 12 at 4608 x 2304
+// bf16). VECTOR: rows and parameters lie on 16 bytes, a lane has vectors
+// lane, lane + L, ...; else elements lane, lane + L, ..., so that any
+// alignment reads shared memory without conflicts.
+template <typename T, int E, int LO, int L, bool VECTOR>
+__global__ void __launch_bounds__(E <= 32 ? 384 : E <= 64 ? 512 : E <= 96 ? 384 : 256, E <= 32 ? 2 : 1)
+forward_kernel(const FwdArgs a, const FwdPlan p) {
+  constexpr int VEC = 16 / (int)sizeof(T), P = Pairs<T>::N, C = E / VEC, G = 32 / L;
+  constexpr int SURE = LO / VEC;                         // vectors that every lane has
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int l = lane % L, sub = lane / L;
+  const int pd = (a.D + 3) & ~3;
+  float* gs = reinterpret_cast<float*>(smem);            // [pd] g, [pd] h
+  float* hs = gs + pd;
+  uint64_t* full = reinterpret_cast<uint64_t*>(hs + pd) + warp * p.stages;
+  uint8_t* ring = smem + ((2 * pd * 4 + warps * p.stages * 8 + 15) & ~15) +
+                  (size_t)warp * p.stages * p.slot_bytes;
+  const int64_t smp = blockIdx.x / p.chunks;
+  const int64_t c0 = (int64_t)(blockIdx.x % p.chunks) * p.chunk_rows;
+  const int64_t c1 = c0 + p.chunk_rows < a.rows_per_mod ? c0 + p.chunk_rows : a.rows_per_mod;
+  const int64_t base = smp * a.rows_per_mod;
+  const T* x = static_cast<const T*>(a.x);
+  // slot s of this warp: rows first .. first + slot_rows of the chunk
+  const auto first_of = [&](int s) { return c0 + ((int64_t)s * warps + warp) * p.slot_rows; };
+  const int64_t groups = c1 > c0 ? (c1 - c0 + p.slot_rows - 1) / p.slot_rows : 0;
+  const int steps = (int)((groups - warp + warps - 1) / warps);
+  const auto fill = [&](int s) {                         // lane 0
+    const int64_t r = base + first_of(s);
+    const int64_t left = base + c1 - r, rows = left < p.slot_rows ? left : p.slot_rows;
+    const int64_t n = (rows - 1) * a.D + a.D;            // one row, or rows that adjoin
+    uint8_t* dst = ring + (size_t)(s % p.stages) * p.slot_bytes;
+    const T* src = x + r * a.xs;
+    const uint32_t bytes = span_bytes(src, n, r + rows == a.M, dst);
+    mbar_arrive_expect_tx(&full[s % p.stages], bytes);
+    if (bytes) bulk_load(dst, span_of(src, n).from, bytes, &full[s % p.stages]);
+  };
+  if (lane == 0) {
+    for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+    for (int s = 0; s < p.stages && s < steps; ++s) fill(s);
+  }
+  const bool params = a.w.p || a.b.p || a.s.p || a.t.p;
+  if (params)
+    for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
+      // VECTOR: four columns of a vector a plane, so that the lanes' 16-byte
+      // reads adjoin (a vector's eight in a row would share banks two by two)
+      const int at = VECTOR ? c % VEC / 4 * (a.D / (VEC / 4)) + c / VEC * 4 + c % 4 : c;
+      combine<T>(a.w, a.b, a.s, a.t, smp, c, gs[at], hs[at]);
+    }
+  __syncthreads();
+  const float inv_d = 1.0f / (float)a.D;
+  const int nvec = a.D / VEC;
+  T* y = static_cast<T*>(a.y);
+  int slot = 0, phase = 0;
+  for (int s = 0; s < steps; ++s) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], phase, GWB_ERR_TIMEOUT_ACT))) {
+      if (lane == 0) drain(full, p.stages, s, min(steps, s + p.stages));
+      return;
+    }
+    const int64_t r0 = base + first_of(s);
+    const int rows = (int)min((int64_t)p.slot_rows, base + c1 - r0);
+    const uint8_t* src = ring + (size_t)slot * p.slot_bytes;
+    if (!VECTOR) src += reinterpret_cast<uintptr_t>(x + r0 * a.xs) & 15u;
+    for (int k0 = 0; k0 < rows; k0 += G) {
+      const int k = k0 + sub;
+      const bool live = k < rows;
+      F2 v[VECTOR ? E / 2 : 1];
+      float e[VECTOR ? 1 : E];
+      F2 acc = f2(0.0f, 0.0f);
+      const T* row = reinterpret_cast<const T*>(src) + (size_t)(live ? k : 0) * a.D;
+      if constexpr (VECTOR) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          F2 u[P];
+          if (c < SURE || l + c * L < nvec) {
+            unpack<T>(*reinterpret_cast<const uint4*>(row + (l + c * L) * VEC), u);
+          } else {
+#pragma unroll
+            for (int j = 0; j < P; ++j) u[j] = f2(0.0f, 0.0f);
+          }
+#pragma unroll
+          for (int j = 0; j < P; ++j) { v[c * P + j] = u[j]; acc = add2(acc, u[j]); }
+        }
+      } else {
+        float part = 0.0f;
+        each<E, LO, L>(a.D, l, [&](int i, int c, bool in) {
+          e[i] = in ? to_f32<T>(row[c]) : 0.0f;
+          part += e[i];
+        });
+        acc = f2(part, 0.0f);
+      }
+      if (k0 + G >= rows) {
+        // the slot is in registers: bring the rows after next
+        __syncwarp();
+        if (lane == 0 && s + p.stages < steps) fill(s + p.stages);
+      }
+      const float mean = lanes_sum<L>(sum2(acc)) * inv_d;
+      const F2 neg = f2(-mean, -mean);
+      acc = f2(0.0f, 0.0f);
+      if constexpr (VECTOR) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (c < SURE || l + c * L < nvec)
+#pragma unroll
+            for (int j = c * P; j < c * P + P; ++j) {
+              v[j] = add2(v[j], neg);
+              acc = fma2(v[j], v[j], acc);
+            }
+      } else {
+        float part = 0.0f;
+        each<E, LO, L>(a.D, l, [&](int i, int, bool in) {
+          e[i] -= mean;
+          if (in) part += e[i] * e[i];
+        });
+        acc = f2(part, 0.0f);
+      }
+      // rsqrtf: 2 ulp, far inside the statistics' own rounding
+      const float rstd = rsqrtf(lanes_sum<L>(sum2(acc)) * inv_d + a.eps);
+      if (!live) continue;
+      const int64_t r = r0 + k;
+      if (l == 0 && a.mean != nullptr) {
+        a.mean[r] = mean;
+        a.rstd[r] = rstd;
+      }
+      const F2 r2 = f2(rstd, rstd);
+      T* out = y + r * a.D;
+      if constexpr (VECTOR) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int i = l + c * L;
+          if (c >= SURE && i >= nvec) continue;
+          F2 u[P];
+#pragma unroll
+          for (int j = 0; j < P; ++j) u[j] = mul2(v[c * P + j], r2);
+          if (params) {
+#pragma unroll
+            for (int j = 0; j < P; j += 2) {
+              const int at = (j / 2) * (a.D / (VEC / 4)) + i * 4;
+              const float4 g4 = *reinterpret_cast<const float4*>(gs + at);
+              const float4 h4 = *reinterpret_cast<const float4*>(hs + at);
+              u[j] = fma2(u[j], f2(g4.x, g4.y), f2(h4.x, h4.y));
+              u[j + 1] = fma2(u[j + 1], f2(g4.z, g4.w), f2(h4.z, h4.w));
+            }
+          }
+          *reinterpret_cast<uint4*>(out + i * VEC) = repack<T>(u);
+        }
+      } else {
+        each<E, LO, L>(a.D, l, [&](int i, int c, bool in) {
+          if (!in) return;
+          const float z = e[i] * rstd;
+          out[c] = from_f32<T>(params ? z * gs[c] + hs[c] : z);
+        });
+      }
+    }
+    if (++slot == p.stages) { slot = 0; phase ^= 1; }
+  }
+}
+
+// Rows of over 4096 elements, one a CTA of 512 threads; the row stays in
 // registers, C vectors a thread, between the statistics and the output.
-template <typename T, int VEC, int C, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 1024)
-forward_kernel(const FwdArgs a) {
+template <typename T, int VEC, int C>
+__global__ void __launch_bounds__(512) forward_block_kernel(const FwdArgs a) {
   __shared__ float red[2][32];
-  const int lanes = WARP ? 32 : blockDim.x;
-  const int t = WARP ? (threadIdx.x & 31) : threadIdx.x;
-  const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  if (WARP && row >= a.M) return;
+  const int lanes = blockDim.x, t = threadIdx.x;
+  const int64_t row = blockIdx.x;
   const int nvec = a.D / VEC;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
   Pack<T, VEC> raw[C];
@@ -109,7 +356,7 @@ forward_kernel(const FwdArgs a) {
       sum += v[c][j];
     }
   const float inv_d = 1.0f / (float)a.D;
-  const float mean = (WARP ? warp_sum(sum) : block_sum(sum, red[0])) * inv_d;
+  const float mean = block_sum(sum, red[0]) * inv_d;
   float sq = 0.0f;
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -119,8 +366,8 @@ forward_kernel(const FwdArgs a) {
         v[c][j] -= mean;
         sq += v[c][j] * v[c][j];
       }
-  const float var = (WARP ? warp_sum(sq) : block_sum(sq, red[1])) * inv_d;
-  const float rstd = 1.0f / sqrtf(var + a.eps);
+  const float var = block_sum(sq, red[1]) * inv_d;
+  const float rstd = rsqrtf(var + a.eps);
   if (t == 0 && a.mean != nullptr) {
     a.mean[row] = mean;
     a.rstd[row] = rstd;
@@ -213,18 +460,13 @@ __device__ __forceinline__ void gain(const Param& w, const Param& s, int64_t smp
   }
 }
 
-// CTA blockIdx.x takes one chunk of one sample's rows. WARP: its eight warps
-// take rows in turn, one row a warp; else the CTA takes R rows at a time and
-// each thread keeps its C vectors of columns, so S1 and S2 stay in its
-// registers for the whole chunk and the 2 R row sums share two barriers.
-template <typename T, int VEC, int C, int R, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512)
-backward_kernel(const BwdArgs a) {
-  extern __shared__ float part_sm[];             // WARP: [8][2][D]
-  __shared__ float red[2][32][2 * R];
-  const int lanes = WARP ? 32 : blockDim.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = WARP ? lane : threadIdx.x;
+// Narrow rows (up to 64 vectors): CTA blockIdx.x takes one chunk of one
+// sample's rows, its eight warps rows in turn, one a warp; a thread keeps its
+// C vectors of columns, joined over the warps at the end.
+template <typename T, int VEC, int C>
+__global__ void __launch_bounds__(256) backward_kernel(const BwdArgs a) {
+  extern __shared__ float part_sm[];             // [8][2][D]
+  const int warp = threadIdx.x >> 5, t = threadIdx.x & 31;
   const int nvec = a.D / VEC;
   const int64_t smp = blockIdx.x / a.chunks;
   const int64_t r0 = (int64_t)(blockIdx.x % a.chunks) * a.chunk_rows;
@@ -236,104 +478,307 @@ backward_kernel(const BwdArgs a) {
   for (int c = 0; c < C; ++c) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) g[c][j] = s1[c][j] = s2[c][j] = 0.0f;
-    if (t + c * lanes < nvec) gain<T, VEC>(a.w, a.s, smp, (t + c * lanes) * VEC, g[c]);
+    if (t + c * 32 < nvec) gain<T, VEC>(a.w, a.s, smp, (t + c * 32) * VEC, g[c]);
   }
-  const int64_t step = WARP ? (int64_t)(blockDim.x >> 5) * R : R;
-  int flip = 0;
-  for (int64_t r = r0 + (WARP ? warp * R : 0); r < r1; r += step, flip ^= 1) {
-    Pack<T, VEC> xv[R][C], dv[R][C];
-    float mean[R], rstd[R];
+  Pack<T, VEC> xn[C], dn[C];                     // the next row's
+  float meann = 0.0f, rstdn = 0.0f;
+  const auto fetch = [&](int64_t r) {
+    const int64_t row = base + r;
+    meann = __ldg(a.mean + row);
+    rstdn = __ldg(a.rstd + row);
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const bool live = r + k < r1;
-      const int64_t row = base + (live ? r + k : r);
-      mean[k] = __ldg(a.mean + row);
-      rstd[k] = __ldg(a.rstd + row);
+    for (int c = 0; c < C; ++c)
+      if (t + c * 32 < nvec) {
+        xn[c].load(static_cast<const T*>(a.x) + row * a.xs + (t + c * 32) * VEC);
+        dn[c].load(static_cast<const T*>(a.dy) + row * a.dys + (t + c * 32) * VEC);
+      }
+  };
+  if (r0 + warp < r1) fetch(r0 + warp);
+  for (int64_t r = r0 + warp; r < r1; r += 8) {
+    Pack<T, VEC> xv[C], dv[C];
+    const float mean = meann, rstd = rstdn;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (t + c * lanes < nvec) {
-          xv[k][c].load(static_cast<const T*>(a.x) + row * a.xs + (t + c * lanes) * VEC);
-          dv[k][c].load(static_cast<const T*>(a.dy) + row * a.dys + (t + c * lanes) * VEC);
+    for (int c = 0; c < C; ++c) { xv[c] = xn[c]; dv[c] = dn[c]; }
+    if (r + 8 < r1) fetch(r + 8);
+    float sa = 0.0f, sb = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (t + c * 32 < nvec)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float z = (xv[c].get(j) - mean) * rstd, d = dv[c].get(j), e = d * z;
+          s1[c][j] += d;
+          s2[c][j] += e;
+          sa += d * g[c][j];
+          sb += e * g[c][j];
         }
+    if (a.dx == nullptr) continue;
+    const float ma = warp_sum(sa) * inv_d, mb = warp_sum(sb) * inv_d;
+    T* dx = static_cast<T*>(a.dx) + (base + r) * a.D;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (t + c * 32 < nvec) {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float z = (xv[c].get(j) - mean) * rstd;
+          o.set(j, rstd * (dv[c].get(j) * g[c][j] - ma - z * mb));
+        }
+        o.store(dx + (t + c * 32) * VEC);
+      }
+  }
+  if (a.partial == nullptr) return;
+  float* mine = part_sm + warp * 2 * a.D;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (t + c * 32 < nvec)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        mine[(t + c * 32) * VEC + j] = s1[c][j];
+        mine[a.D + (t + c * 32) * VEC + j] = s2[c][j];
+      }
+  __syncthreads();
+  float* out = a.partial + (int64_t)blockIdx.x * 2 * a.D;
+  for (int i = threadIdx.x; i < 2 * a.D; i += blockDim.x) {
+    float v = 0.0f;
+    for (int w = 0; w < 8; ++w) v += part_sm[w * 2 * a.D + i];
+    out[i] = v;
+  }
+}
+
+// Sums N values (a power of two, at most 8) over the warp's lanes in N - 1 +
+// 5 - log2 N shuffles rather than 5 N: each step halves the values a lane
+// carries. Returns the sum of value (lane >> (5 - log2 N)); fixed order.
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  int half = 16;
+#pragma unroll
+  for (int n = N; n > 1; n /= 2, half /= 2) {
+    const bool up = lane & half;
+#pragma unroll
+    for (int k = 0; k < n / 2; ++k) {
+      const float keep = up ? v[k + n / 2] : v[k], give = up ? v[k] : v[k + n / 2];
+      v[k] = keep + __shfl_xor_sync(0xffffffffu, give, half);
     }
-    float sa[R], sb[R];
+  }
+#pragma unroll
+  for (; half; half /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], half);
+  return v[0];
+}
+
+struct BwdPlan { int stages; uint32_t x_slot; int64_t last; };
+
+// One CTA per chunk of one sample's rows. Bulk copies bring two rows of x and
+// dy at a time into a ring of slots, far enough ahead that reading never
+// waits for the row sums' barrier. A thread keeps its E columns of the gain
+// and of both column sums in registers for the whole chunk; the second pass
+// over a slot (dx) reads it from shared memory again, because holding it would
+// halve the warps a multiprocessor runs, and their number is what hides the
+// latencies here (a form with 16 columns a thread and half the warps took 115
+// us against 94 at 18432 x 2304 bf16). A slot is filled again after the next
+// step's barrier. Every wait is bounded, and all threads leave together.
+template <typename T, int E, bool VECTOR>
+__global__ void __launch_bounds__(E <= 8 ? 384 : 512, E <= 8 ? 2 : 1)
+backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
+  constexpr int R = 2, VEC = 16 / (int)sizeof(T), P = Pairs<T>::N, C = E / VEC;
+  extern __shared__ __align__(16) uint8_t ring[];        // [stages][R][x, dy]
+  __shared__ float red[2][16][2 * R];
+  __shared__ __align__(8) uint64_t full[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = threadIdx.x;
+  const int lanes = blockDim.x, nw = blockDim.x >> 5, nvec = a.D / VEC;
+  const int64_t smp = blockIdx.x / a.chunks;
+  const int64_t r0 = (int64_t)(blockIdx.x % a.chunks) * a.chunk_rows;
+  const int count = (int)max((int64_t)0, min(a.chunk_rows, a.rows_per_mod - r0));
+  const int64_t base = smp * a.rows_per_mod + r0;
+  const int steps = (count + R - 1) / R;
+  const uint32_t slot_bytes = 2 * R * p.x_slot;
+  const float inv_d = 1.0f / (float)a.D;
+  const T* x = static_cast<const T*>(a.x) + base * a.xs;
+  const T* dy = static_cast<const T*>(a.dy) + base * a.dys;
+  const auto fill = [&](int s, int slot) {               // thread 0
+    uint8_t* dst = ring + slot * slot_bytes;
+    uint32_t bytes[2 * R];
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-      sa[k] = sb[k] = 0.0f;
-      if (r + k < r1)
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-          if (t + c * lanes < nvec)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              const float z = (xv[k][c].get(j) - mean[k]) * rstd[k], d = dv[k][c].get(j);
-              s1[c][j] += d;
-              s2[c][j] += d * z;
-              const float i = d * g[c][j];
-              sa[k] += i;
-              sb[k] += i * z;
-            }
+      const int r = s * R + k;
+      bytes[2 * k] = bytes[2 * k + 1] = 0;
+      if (r < count) {
+        const bool last = base + r == p.last;
+        bytes[2 * k] = span_bytes(x + r * a.xs, a.D, last, dst + 2 * k * p.x_slot);
+        bytes[2 * k + 1] = span_bytes(dy + r * a.dys, a.D, last, dst + (2 * k + 1) * p.x_slot);
+      }
     }
-    if (a.dx == nullptr) continue;
+    mbar_arrive_expect_tx(&full[slot], bytes[0] + bytes[1] + bytes[2] + bytes[3]);
 #pragma unroll
-    for (int k = 0; k < R; ++k) { sa[k] = warp_sum(sa[k]); sb[k] = warp_sum(sb[k]); }
-    if constexpr (!WARP) {
-      if (lane == 0)
+    for (int k = 0; k < R; ++k) {
+      const int r = s * R + k;
+      if (bytes[2 * k])
+        bulk_load(dst + 2 * k * p.x_slot, span_of(x + r * a.xs, a.D).from, bytes[2 * k], &full[slot]);
+      if (bytes[2 * k + 1])
+        bulk_load(dst + (2 * k + 1) * p.x_slot, span_of(dy + r * a.dys, a.D).from, bytes[2 * k + 1],
+                  &full[slot]);
+    }
+  };
+  if (t == 0) {
+    for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (t == 0)
+    for (int s = 0; s < p.stages && s < steps; ++s) fill(s, s);
+  // columns: vectors t, t + lanes, ... or elements t, t + lanes, ...
+  const F2 zero = f2(0.0f, 0.0f);
+  F2 g[E / 2], s1[E / 2], s2[E / 2];
 #pragma unroll
-        for (int k = 0; k < R; ++k) { red[flip][warp][2 * k] = sa[k]; red[flip][warp][2 * k + 1] = sb[k]; }
-      __syncthreads();
-      const int nw = blockDim.x >> 5;
+  for (int j = 0; j < E / 2; ++j) {
+    float gv[2];
 #pragma unroll
-      for (int k = 0; k < R; ++k) {
-        sa[k] = warp_sum(lane < nw ? red[flip][lane][2 * k] : 0.0f);
-        sb[k] = warp_sum(lane < nw ? red[flip][lane][2 * k + 1] : 0.0f);
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * j + e;
+      const int col = VECTOR ? (t + i / VEC * lanes) * VEC + i % VEC : t + i * lanes;
+      float h;
+      gv[e] = 0.0f;
+      if (col < a.D) combine<T>(a.w, {}, a.s, {}, smp, col, gv[e], h);
+    }
+    g[j] = f2(gv[0], gv[1]);
+    s1[j] = s2[j] = zero;
+  }
+  // z and d of one row of a slot, E columns of this thread; absent ones give
+  // z = d = 0
+  const auto values = [&](const uint8_t* src, uint32_t xl, uint32_t dl, F2 neg, F2 r2, int c,
+                          F2 (&z)[P], F2 (&d)[P]) {
+    if constexpr (VECTOR) {
+      unpack<T>(*reinterpret_cast<const uint4*>(src + (t + c * lanes) * 16), z);
+      unpack<T>(*reinterpret_cast<const uint4*>(src + p.x_slot + (t + c * lanes) * 16), d);
+    } else {
+      const T* xr = reinterpret_cast<const T*>(src + xl);
+      const T* dr = reinterpret_cast<const T*>(src + p.x_slot + dl);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        float xv[2], dv[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = t + (c * VEC + 2 * j + e) * lanes;
+          const float2 n = split(neg);
+          xv[e] = col < a.D ? to_f32<T>(xr[col]) : -n.x;
+          dv[e] = col < a.D ? to_f32<T>(dr[col]) : 0.0f;
+        }
+        z[j] = f2(xv[0], xv[1]);
+        d[j] = f2(dv[0], dv[1]);
       }
     }
 #pragma unroll
+    for (int j = 0; j < P; ++j) z[j] = mul2(add2(z[j], neg), r2);
+  };
+  float mean[R], rstd[R], mean1[R], rstd1[R];            // of this step, of the next
+  const auto stats = [&](int s) {
+#pragma unroll
     for (int k = 0; k < R; ++k) {
-      if (r + k >= r1) continue;
-      const float ma = sa[k] * inv_d, mb = sb[k] * inv_d;
-      T* dx = static_cast<T*>(a.dx) + (base + r + k) * a.D;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (t + c * lanes < nvec) {
-          Pack<T, VEC> o;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float z = (xv[k][c].get(j) - mean[k]) * rstd[k];
-            o.set(j, rstd[k] * (dv[k][c].get(j) * g[c][j] - ma - z * mb));
-          }
-          o.store(dx + (t + c * lanes) * VEC);
-        }
+      const int r = min(s * R + k, count - 1);
+      mean1[k] = __ldg(a.mean + base + r);
+      rstd1[k] = __ldg(a.rstd + base + r);
     }
+  };
+  if (steps) stats(0);
+  int s = 0, slot = 0, freed = 0, phase = 0, filled = min(steps, p.stages);
+  for (; s < steps; ++s) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) { mean[k] = mean1[k]; rstd[k] = rstd1[k]; }
+    if (s + 1 < steps) stats(s + 1);
+    const bool ok = mbar_wait(&full[slot], phase, GWB_ERR_TIMEOUT_ACT);
+    const uint8_t* src = ring + slot * slot_bytes;
+    const int rows = min(R, count - s * R);
+    uint32_t xl[R], dl[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      xl[k] = VECTOR ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(x + (int64_t)(s * R + k) * a.xs) & 15u);
+      dl[k] = VECTOR ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(dy + (int64_t)(s * R + k) * a.dys) & 15u);
+    }
+    float sums[2 * R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      F2 sa = zero, sb = zero;
+      const F2 neg = f2(-mean[k], -mean[k]), r2 = f2(rstd[k], rstd[k]);
+      if (k < rows)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          if (VECTOR && t + c * lanes >= nvec) continue;
+          F2 z[P], d[P];
+          values(src + 2 * k * p.x_slot, xl[k], dl[k], neg, r2, c, z, d);
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            const F2 e = mul2(d[j], z[j]);
+            s1[c * P + j] = add2(s1[c * P + j], d[j]);
+            s2[c * P + j] = add2(s2[c * P + j], e);
+            sa = fma2(d[j], g[c * P + j], sa);
+            sb = fma2(e, g[c * P + j], sb);
+          }
+        }
+      sums[2 * k] = sum2(sa);
+      sums[2 * k + 1] = sum2(sb);
+    }
+    const float mine = warp_sums<2 * R>(sums);
+    if ((lane & 7) == 0) red[s & 1][warp][lane >> 3] = mine;
+    if (!__syncthreads_and(ok)) break;
+    // every thread is past the second pass of step s - 1
+    if (s > 0 && filled < steps) {
+      if (t == 0) fill(filled, freed);
+      if (++freed == p.stages) freed = 0;
+      ++filled;
+    }
+    if (a.dx != nullptr) {
+      // lanes 8 v .. 8 v + 7 add value v's warp sums, then hand the total round
+      float v = (lane & 7) < nw ? red[s & 1][lane & 7][lane >> 3] : 0.0f;
+      if ((lane & 7) + 8 < nw) v += red[s & 1][(lane & 7) + 8][lane >> 3];
+#pragma unroll
+      for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const float ma = -__shfl_sync(0xffffffffu, v, 16 * k) * inv_d * rstd[k];
+        const float mb = -__shfl_sync(0xffffffffu, v, 16 * k + 8) * inv_d * rstd[k];
+        if (k >= rows) continue;
+        const F2 neg = f2(-mean[k], -mean[k]), r2 = f2(rstd[k], rstd[k]);
+        const F2 ma2 = f2(ma, ma), mb2 = f2(mb, mb);
+        T* dx = static_cast<T*>(a.dx) + (base + s * R + k) * a.D;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          if (VECTOR && t + c * lanes >= nvec) continue;
+          F2 z[P], d[P];
+          values(src + 2 * k * p.x_slot, xl[k], dl[k], neg, r2, c, z, d);
+#pragma unroll
+          for (int j = 0; j < P; ++j)
+            d[j] = fma2(z[j], mb2, fma2(mul2(d[j], g[c * P + j]), r2, ma2));
+          if constexpr (VECTOR) {
+            *reinterpret_cast<uint4*>(dx + (t + c * lanes) * VEC) = repack<T>(d);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              const int col = t + (c * VEC + j) * lanes;
+              const float2 f = split(d[j / 2]);
+              if (col < a.D) dx[col] = from_f32<T>(j & 1 ? f.y : f.x);
+            }
+          }
+        }
+      }
+    }
+    if (++slot == p.stages) { slot = 0; phase ^= 1; }
+  }
+  if (s < steps) {
+    if (t == 0) drain(full, p.stages, s, filled);
+    __syncthreads();
+    return;
   }
   if (a.partial == nullptr) return;
   float* out = a.partial + (int64_t)blockIdx.x * 2 * a.D;
-  if constexpr (WARP) {
-    float* mine = part_sm + warp * 2 * a.D;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (t + c * lanes < nvec)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          mine[(t + c * lanes) * VEC + j] = s1[c][j];
-          mine[a.D + (t + c * lanes) * VEC + j] = s2[c][j];
-        }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * a.D; i += blockDim.x) {
-      float v = 0.0f;
-      for (int w = 0; w < (int)(blockDim.x >> 5); ++w) v += part_sm[w * 2 * a.D + i];
-      out[i] = v;
+  for (int i = 0; i < E; ++i) {
+    const int col = VECTOR ? (t + i / VEC * lanes) * VEC + i % VEC : t + i * lanes;
+    const float2 u = split(s1[i / 2]), v = split(s2[i / 2]);
+    if (col < a.D) {
+      out[col] = i & 1 ? u.y : u.x;
+      out[a.D + col] = i & 1 ? v.y : v.x;
     }
-  } else {
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (t + c * lanes < nvec)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          out[(t + c * lanes) * VEC + j] = s1[c][j];
-          out[a.D + (t + c * lanes) * VEC + j] = s2[c][j];
-        }
   }
 }
 
@@ -461,83 +906,135 @@ bool vector_ok(int D, std::initializer_list<const void*> ptrs, std::initializer_
   return true;
 }
 
-template <typename T, int VEC, int C>
-int forward_c(const FwdArgs& a, int th, cudaStream_t st) {
-  if (th == 32) forward_kernel<T, VEC, C, true><<<(unsigned)((a.M + 3) / 4), 128, 0, st>>>(a);
-  else forward_kernel<T, VEC, C, false><<<(unsigned)a.M, th, 0, st>>>(a);
+template <typename T, int E, int LO, int L, bool VECTOR>
+int forward_l(FwdArgs a, cudaStream_t st) {
+  auto kern = forward_kernel<T, E, LO, L, VECTOR>;
+  constexpr int most_warps = E <= 32 ? 12 : E <= 64 ? 16 : E <= 96 ? 12 : 8, per_sm = E <= 32 ? 2 : 1;
+  const bool mod = a.s.p || a.t.p;
+  if (!mod) a.rows_per_mod = a.M;
+  const int64_t samples = a.M / a.rows_per_mod;
+  FwdPlan p;
+  // a copy brings one row, or several that adjoin up to 4 KB (small copies
+  // cost their issue, not their bytes), as long as every warp gets one
+  const int row = a.D * (int)sizeof(T), sms = sm_count();
+  p.slot_rows = 1;
+  if (a.xs == a.D) {
+    while (p.slot_rows < 16 && 2 * p.slot_rows * row <= 4096 &&
+           a.M / (2 * p.slot_rows) >= (int64_t)sms * per_sm * most_warps)
+      p.slot_rows *= 2;
+    if (a.M >= 32 / L && p.slot_rows < 32 / L) p.slot_rows = 32 / L;
+  }
+  p.slot_bytes = (uint32_t)(p.slot_rows * row + 15 + 15) / 16 * 16;
+  const int fixed = 2 * ((a.D + 3) & ~3) * 4 + 16 * 8 * 8 + 16;
+  const int room = 225 * 1024 / per_sm - 1024 - fixed;
+  int warps = most_warps;
+  const int64_t groups = (a.rows_per_mod + p.slot_rows - 1) / p.slot_rows;
+  // two slots a warp at least: one read, one in flight
+  while (warps > 1 && warps * 2 * (int)p.slot_bytes > room) --warps;
+  while (warps > 1 && samples * ((groups + warps - 1) / warps) < (int64_t)sms * per_sm) --warps;
+  p.stages = std::max(2, std::min(4, room / (warps * (int)p.slot_bytes)));
+  const int64_t most = (groups + warps - 1) / warps;
+  const int64_t want = ((int64_t)sms * per_sm + samples - 1) / samples;
+  const int64_t chunks = std::max<int64_t>(1, std::min(most, want));
+  p.chunk_rows = (groups + chunks - 1) / chunks * p.slot_rows;
+  p.chunks = (int)((a.rows_per_mod + p.chunk_rows - 1) / p.chunk_rows);
+  const int64_t blocks = samples * p.chunks;
+  if (blocks > 0x7fffffff) return GWB_E_CAPACITY;
+  const size_t smem = ((2 * ((a.D + 3) & ~3) * 4 + warps * p.stages * 8 + 15) & ~15) +
+                      (size_t)warps * p.stages * p.slot_bytes;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+      cudaSuccess)
+    return GWB_E_LAUNCH;
+  kern<<<(unsigned)blocks, warps * 32, smem, st>>>(a, p);
   return launch_status();
 }
 
-// Threads a row: the fewest warps that keep a thread at four vectors (one
-// warp needs no barrier; more rows in flight beat more threads a row), the
-// register file's limit being 1024 threads.
-template <typename T, int VEC>
+// Lanes a row: eight up to 64 elements (four rows a warp), else 32, with the
+// fewest elements a lane that cover it.
+template <typename T, bool VECTOR>
 int forward_v(const FwdArgs& a, cudaStream_t st) {
-  constexpr int CMAX = VEC == 1 ? 8 : 4;
-  const int nvec = a.D / VEC;
-  int th = 32;
-  while (th < 1024 && nvec > th * CMAX) th *= 2;
-  if (nvec > th * CMAX) {
-    forward_wide_kernel<T><<<(unsigned)a.M, 1024, 0, st>>>(a);
-    return launch_status();
-  }
-  const int c = (nvec + th - 1) / th;
-  if (c <= 1) return forward_c<T, VEC, 1>(a, th, st);
-  if (c <= 2) return forward_c<T, VEC, 2>(a, th, st);
-  if (c <= 3) return forward_c<T, VEC, 3>(a, th, st);
-  if (c <= 4) return forward_c<T, VEC, 4>(a, th, st);
-  if constexpr (CMAX > 4) return forward_c<T, VEC, 8>(a, th, st);
-  return GWB_E_SHAPE;
+  if (a.D <= 64) return forward_l<T, 8, 0, 8, VECTOR>(a, st);
+  const int e = (a.D + 31) / 32;
+  if (a.D <= 128) return forward_l<T, 16, 8, 8, VECTOR>(a, st);
+  if (e <= 8) return forward_l<T, 8, 4, 32, VECTOR>(a, st);
+  if (e <= 16) return forward_l<T, 16, 8, 32, VECTOR>(a, st);
+  if (e <= 24) return forward_l<T, 24, 16, 32, VECTOR>(a, st);
+  if (e <= 32) return forward_l<T, 32, 24, 32, VECTOR>(a, st);
+  if (e <= 48) return forward_l<T, 48, 32, 32, VECTOR>(a, st);
+  if (e <= 64) return forward_l<T, 64, 48, 32, VECTOR>(a, st);
+  if (e <= 96) return forward_l<T, 96, 64, 32, VECTOR>(a, st);
+  if (e <= 128) return forward_l<T, 128, 96, 32, VECTOR>(a, st);
+  constexpr int V = VECTOR ? 16 / (int)sizeof(T) : 1;
+  const int c = (a.D / V + 511) / 512;
+  const bool mod_ok = !VECTOR || vector_ok<T>(a.D, {}, {}, {a.w, a.b, a.s, a.t});
+  if (mod_ok && c <= 2) forward_block_kernel<T, V, 2><<<(unsigned)a.M, 512, 0, st>>>(a);
+  else if (mod_ok && c <= 4) forward_block_kernel<T, V, 4><<<(unsigned)a.M, 512, 0, st>>>(a);
+  else if (!VECTOR && c <= 16) forward_block_kernel<T, 1, 16><<<(unsigned)a.M, 512, 0, st>>>(a);
+  else forward_wide_kernel<T><<<(unsigned)a.M, 1024, 0, st>>>(a);
+  return launch_status();
 }
 
 template <typename T>
 int forward_t(const FwdArgs& a, cudaStream_t st) {
-  if (vector_ok<T>(a.D, {a.x, a.y}, {a.xs}, {a.w, a.b, a.s, a.t}))
-    return forward_v<T, 16 / (int)sizeof(T)>(a, st);
-  return forward_v<T, 1>(a, st);
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool vector = a.D % V == 0 && a.xs % V == 0 && aligned16(a.x) && aligned16(a.y);
+  return vector ? forward_v<T, true>(a, st) : forward_v<T, false>(a, st);
 }
 
-template <typename T, int VEC, int C, bool WARP>
-int backward_c(const BwdArgs& a, int64_t blocks, int th, cudaStream_t st) {
-  // rows a step: as many as keep x, dy, the gain and both sums in the 128
-  // registers that 512 threads leave each other
-  constexpr int E = VEC * C, WIDE = sizeof(T) == 4 || VEC == 1;
-  constexpr int R = WARP ? 1 : E <= 4 ? 4 : E <= 8 ? (WIDE ? 2 : 4) : (WIDE ? 1 : 2);
-  const size_t smem = WARP && a.partial ? (size_t)8 * 2 * a.D * sizeof(float) : 0;
-  backward_kernel<T, VEC, C, R, WARP><<<(unsigned)blocks, th, smem, st>>>(a);
+template <typename T, int VEC, int C>
+int backward_c(const BwdArgs& a, int64_t blocks, cudaStream_t st) {
+  const size_t smem = a.partial ? (size_t)8 * 2 * a.D * sizeof(float) : 0;
+  backward_kernel<T, VEC, C><<<(unsigned)blocks, 256, smem, st>>>(a);
   return launch_status();
+}
+
+template <typename T, int E, bool VECTOR>
+int backward_staged_e(const BwdArgs& a, int64_t blocks, int64_t rows, int th, cudaStream_t st) {
+  auto kern = backward_staged_kernel<T, E, VECTOR>;
+  // the CTAs that the register file holds share the shared memory: three
+  // slots at least (one read, one being freed, one in flight)
+  const int per_sm = std::max(1, std::min(8, 65536 / (th * (E <= 8 ? 80 : 128))));
+  BwdPlan p;
+  p.x_slot = (uint32_t)(a.D * (int)sizeof(T) + 15 + 15) / 16 * 16;
+  p.last = rows - 1;
+  const int slot = 4 * (int)p.x_slot;
+  p.stages = std::max(3, std::min(8, (220 * 1024 / per_sm - 2048) / slot));
+  const size_t smem = (size_t)p.stages * slot;
+  if (smem > 226 * 1024) return GWB_E_SHAPE;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+      cudaSuccess)
+    return GWB_E_LAUNCH;
+  kern<<<(unsigned)blocks, th, smem, st>>>(a, p);
+  return launch_status();
+}
+
+// Eight columns a thread up to 384 threads, then sixteen; rows whose three
+// slots pass the shared memory take the wide form.
+inline bool staged_fits(int D, int size) { return D <= 8192 && 3 * 4 * (D * size + 30) <= 226 * 1024; }
+template <typename T, bool VECTOR>
+int backward_staged(const BwdArgs& a, int64_t blocks, int64_t rows, cudaStream_t st) {
+  const int unit = (a.D + 7) / 8;
+  if (unit <= 384)
+    return backward_staged_e<T, 8, VECTOR>(a, blocks, rows, (unit + 31) / 32 * 32, st);
+  return backward_staged_e<T, 16, VECTOR>(a, blocks, rows, ((a.D + 15) / 16 + 31) / 32 * 32, st);
 }
 
 template <typename T, int VEC>
 int backward_v(const BwdArgs& a, int64_t samples, cudaStream_t st) {
-  const int64_t blocks = samples * a.chunks;
+  const int64_t blocks = samples * a.chunks, rows = samples * a.rows_per_mod;
   const int nvec = a.D / VEC;
-  constexpr int E = 16 / VEC;        // columns a thread: at most 16
-  if (nvec > 512 * E) {
-    if (a.dx) {
-      backward_wide_kernel<T><<<(unsigned)(samples * a.rows_per_mod), 1024, 0, st>>>(a);
-      if (int rc = launch_status()) return rc;
-    }
-    if (a.partial) {
-      backward_wide_sums_kernel<T><<<dim3((unsigned)blocks, (a.D + 31) / 32), 256, 0, st>>>(a);
-      return launch_status();
-    }
-    return GWB_SUCCESS;
+  if (nvec <= 32) return backward_c<T, VEC, 1>(a, blocks, st);
+  if (nvec <= 64) return backward_c<T, VEC, 2>(a, blocks, st);
+  if (staged_fits(a.D, sizeof(T))) return backward_staged<T, (VEC > 1)>(a, blocks, rows, st);
+  if (a.dx) {
+    backward_wide_kernel<T><<<(unsigned)rows, 1024, 0, st>>>(a);
+    if (int rc = launch_status()) return rc;
   }
-  if (nvec <= 32) return backward_c<T, VEC, 1, true>(a, blocks, 256, st);
-  if (nvec <= 64) return backward_c<T, VEC, 2, true>(a, blocks, 256, st);
-  int c = 1;
-  while (nvec > 512 * c) c *= 2;
-  const int th = ((nvec + c - 1) / c + 31) / 32 * 32;
-  if (c == 1) return backward_c<T, VEC, 1, false>(a, blocks, th, st);
-  if (c == 2) return backward_c<T, VEC, 2, false>(a, blocks, th, st);
-  if constexpr (E >= 4)
-    if (c == 4) return backward_c<T, VEC, 4, false>(a, blocks, th, st);
-  if constexpr (E >= 8)
-    if (c == 8) return backward_c<T, VEC, 8, false>(a, blocks, th, st);
-  if constexpr (E >= 16)
-    if (c == 16) return backward_c<T, VEC, 16, false>(a, blocks, th, st);
-  return GWB_E_SHAPE;
+  if (a.partial) {
+    backward_wide_sums_kernel<T><<<dim3((unsigned)blocks, (a.D + 31) / 32), 256, 0, st>>>(a);
+    return launch_status();
+  }
+  return GWB_SUCCESS;
 }
 
 template <typename T>
@@ -557,12 +1054,13 @@ int backward_t(const BwdArgs& a, int64_t samples, const SumArgs& sums, bool want
   return launch_status();
 }
 
-// Chunks a sample's rows are split into for the backward pass: four CTAs a
-// multiprocessor over all samples (their barriers then overlap), no chunk
-// under eight rows (below that the partials outweigh the rows).
-inline int chunks_of(int64_t samples, int64_t rows_per_mod) {
+// Chunks a sample's rows are split into for the backward pass: over all
+// samples as many CTAs as run at once (two a multiprocessor for wide rows,
+// four for narrow ones), no chunk under eight rows (below that the partials
+// outweigh the rows).
+inline int chunks_of(int64_t samples, int64_t rows_per_mod, int64_t D) {
   if (samples <= 0 || rows_per_mod <= 0) return 1;
-  const int64_t want = (148 * 4 + samples - 1) / samples;
+  const int64_t want = (148 * (D > 1536 ? 2 : 4) + samples - 1) / samples;
   const int64_t most = (rows_per_mod + 7) / 8;
   const int64_t c = want < most ? want : most;
   return (int)(c < 1 ? 1 : c);
