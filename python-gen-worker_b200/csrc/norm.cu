@@ -579,14 +579,14 @@ struct BwdPlan { int stages; uint32_t x_slot; int64_t last; };
 // us against 94 at 18432 x 2304 bf16). A slot is filled again after the next
 // step's barrier. Every wait is bounded, and all threads leave together.
 template <typename T, int E, bool VECTOR>
-__global__ void __launch_bounds__(E <= 8 ? 384 : 512, E <= 8 ? 2 : 1)
+__global__ void __launch_bounds__(E <= 8 ? 416 : E <= 16 ? 512 : 384, E <= 8 ? 2 : 1)
 backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
   constexpr int R = 2, VEC = 16 / (int)sizeof(T), P = Pairs<T>::N, C = E / VEC;
   extern __shared__ __align__(16) uint8_t ring[];        // [stages][R][x, dy]
   __shared__ float red[2][16][2 * R];
   __shared__ __align__(8) uint64_t full[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = threadIdx.x;
-  const int lanes = blockDim.x, nw = blockDim.x >> 5, nvec = a.D / VEC;
+  const int lanes = blockDim.x - 32, nw = lanes >> 5, nvec = a.D / VEC;   // the last warp copies
   const int64_t smp = blockIdx.x / a.chunks;
   const int64_t r0 = (int64_t)(blockIdx.x % a.chunks) * a.chunk_rows;
   const int count = (int)max((int64_t)0, min(a.chunk_rows, a.rows_per_mod - r0));
@@ -596,38 +596,44 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
   const float inv_d = 1.0f / (float)a.D;
   const T* x = static_cast<const T*>(a.x) + base * a.xs;
   const T* dy = static_cast<const T*>(a.dy) + base * a.dys;
-  const auto fill = [&](int s, int slot) {               // thread 0
-    uint8_t* dst = ring + slot * slot_bytes;
-    uint32_t bytes[2 * R];
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int r = s * R + k;
-      bytes[2 * k] = bytes[2 * k + 1] = 0;
-      if (r < count) {
-        const bool last = base + r == p.last;
-        bytes[2 * k] = span_bytes(x + r * a.xs, a.D, last, dst + 2 * k * p.x_slot);
-        bytes[2 * k + 1] = span_bytes(dy + r * a.dys, a.D, last, dst + (2 * k + 1) * p.x_slot);
-      }
-    }
-    mbar_arrive_expect_tx(&full[slot], bytes[0] + bytes[1] + bytes[2] + bytes[3]);
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int r = s * R + k;
-      if (bytes[2 * k])
-        bulk_load(dst + 2 * k * p.x_slot, span_of(x + r * a.xs, a.D).from, bytes[2 * k], &full[slot]);
-      if (bytes[2 * k + 1])
-        bulk_load(dst + (2 * k + 1) * p.x_slot, span_of(dy + r * a.dys, a.D).from, bytes[2 * k + 1],
-                  &full[slot]);
-    }
+  // lanes 0 .. 2 R - 1 of the copying warp: row lane / 2 of x or dy each
+  const auto fill = [&](int s, int slot) {
+    const int r = s * R + (lane >> 1);
+    const T* src = lane & 1 ? dy + r * a.dys : x + r * a.xs;
+    uint8_t* dst = ring + slot * slot_bytes + lane * p.x_slot;
+    const uint32_t bytes = r < count ? span_bytes(src, a.D, base + r == p.last, dst) : 0u;
+    mbar_arrive_expect_tx(&full[slot], bytes);
+    if (bytes) bulk_load(dst, span_of(src, a.D).from, bytes, &full[slot]);
   };
   if (t == 0) {
-    for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 2 * R);
     fence_barrier_init();
   }
   __syncthreads();
-  if (t == 0)
-    for (int s = 0; s < p.stages && s < steps; ++s) fill(s, s);
-  // columns: vectors t, t + lanes, ... or elements t, t + lanes, ...
+  if (warp == nw) {
+    // a warp of its own, or the others would wait for it while it works out
+    // addresses
+    int filled = min(steps, p.stages), freed = 0, s = 0;
+    if (lane < 2 * R)
+      for (int k = 0; k < filled; ++k) fill(k, k);
+    for (; s < steps; ++s) {
+      if (!__syncthreads_and(1)) break;
+      // every thread is past the second pass of step s - 1
+      if (s > 0 && filled < steps) {
+        if (lane < 2 * R) fill(filled, freed);
+        if (++freed == p.stages) freed = 0;
+        ++filled;
+      }
+    }
+    // a wait ran out: let the copies in flight land before this CTA ends
+    if (s < steps && lane == 0) drain(full, p.stages, s, filled);
+    return;
+  }
+  // columns: vectors t, t + lanes, ..., or 32 E to a warp with its lanes side
+  // by side (the offsets between a lane's elements are then constants, and
+  // only the last warp has any missing)
+  const int col0 = warp * (32 * E) + lane;
+  const bool whole = warp * (32 * E) + 32 * E <= a.D;
   const F2 zero = f2(0.0f, 0.0f);
   F2 g[E / 2], s1[E / 2], s2[E / 2];
 #pragma unroll
@@ -636,7 +642,7 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = 2 * j + e;
-      const int col = VECTOR ? (t + i / VEC * lanes) * VEC + i % VEC : t + i * lanes;
+      const int col = VECTOR ? (t + i / VEC * lanes) * VEC + i % VEC : col0 + 32 * i;
       float h;
       gv[e] = 0.0f;
       if (col < a.D) combine<T>(a.w, {}, a.s, {}, smp, col, gv[e], h);
@@ -644,32 +650,26 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
     g[j] = f2(gv[0], gv[1]);
     s1[j] = s2[j] = zero;
   }
-  // z and d of one row of a slot, E columns of this thread; absent ones give
-  // z = d = 0
-  const auto values = [&](const uint8_t* src, uint32_t xl, uint32_t dl, F2 neg, F2 r2, int c,
-                          F2 (&z)[P], F2 (&d)[P]) {
+  // one vector's worth of columns of a row in a slot; absent ones give `none`
+  const auto read = [&](const uint8_t* row, uint32_t lead, int c, float none, F2 (&v)[P]) {
     if constexpr (VECTOR) {
-      unpack<T>(*reinterpret_cast<const uint4*>(src + (t + c * lanes) * 16), z);
-      unpack<T>(*reinterpret_cast<const uint4*>(src + p.x_slot + (t + c * lanes) * 16), d);
+      unpack<T>(*reinterpret_cast<const uint4*>(row + (t + c * lanes) * 16), v);
     } else {
-      const T* xr = reinterpret_cast<const T*>(src + xl);
-      const T* dr = reinterpret_cast<const T*>(src + p.x_slot + dl);
+      const T* r = reinterpret_cast<const T*>(row + lead) + col0;
+      const int at = 32 * c * VEC;
+      if (whole) {
 #pragma unroll
-      for (int j = 0; j < P; ++j) {
-        float xv[2], dv[2];
+        for (int j = 0; j < P; ++j)
+          v[j] = f2(to_f32<T>(r[at + 64 * j]), to_f32<T>(r[at + 64 * j + 32]));
+      } else {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int col = t + (c * VEC + 2 * j + e) * lanes;
-          const float2 n = split(neg);
-          xv[e] = col < a.D ? to_f32<T>(xr[col]) : -n.x;
-          dv[e] = col < a.D ? to_f32<T>(dr[col]) : 0.0f;
+        for (int j = 0; j < P; ++j) {
+          const int k = at + 64 * j;
+          v[j] = f2(col0 + k < a.D ? to_f32<T>(r[k]) : none,
+                    col0 + k + 32 < a.D ? to_f32<T>(r[k + 32]) : none);
         }
-        z[j] = f2(xv[0], xv[1]);
-        d[j] = f2(dv[0], dv[1]);
       }
     }
-#pragma unroll
-    for (int j = 0; j < P; ++j) z[j] = mul2(add2(z[j], neg), r2);
   };
   float mean[R], rstd[R], mean1[R], rstd1[R];            // of this step, of the next
   const auto stats = [&](int s) {
@@ -681,8 +681,7 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
     }
   };
   if (steps) stats(0);
-  int s = 0, slot = 0, freed = 0, phase = 0, filled = min(steps, p.stages);
-  for (; s < steps; ++s) {
+  for (int s = 0, slot = 0, phase = 0; s < steps; ++s) {
 #pragma unroll
     for (int k = 0; k < R; ++k) { mean[k] = mean1[k]; rstd[k] = rstd1[k]; }
     if (s + 1 < steps) stats(s + 1);
@@ -695,6 +694,9 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
       xl[k] = VECTOR ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(x + (int64_t)(s * R + k) * a.xs) & 15u);
       dl[k] = VECTOR ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(dy + (int64_t)(s * R + k) * a.dys) & 15u);
     }
+    // With p = d (x - mean): S1 += d, S2 += p rstd; sum(i) = sum(d g) and
+    // sum(i z) = rstd sum(p g).
+    F2 dd[R][VECTOR ? E / 2 : 1];      // d, kept for the second pass where registers allow
     float sums[2 * R];
 #pragma unroll
     for (int k = 0; k < R; ++k) {
@@ -704,29 +706,26 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           if (VECTOR && t + c * lanes >= nvec) continue;
-          F2 z[P], d[P];
-          values(src + 2 * k * p.x_slot, xl[k], dl[k], neg, r2, c, z, d);
+          F2 xv[P], dv[P];
+          read(src + 2 * k * p.x_slot, xl[k], c, mean[k], xv);
+          read(src + (2 * k + 1) * p.x_slot, dl[k], c, 0.0f, dv);
 #pragma unroll
           for (int j = 0; j < P; ++j) {
-            const F2 e = mul2(d[j], z[j]);
-            s1[c * P + j] = add2(s1[c * P + j], d[j]);
-            s2[c * P + j] = add2(s2[c * P + j], e);
-            sa = fma2(d[j], g[c * P + j], sa);
-            sb = fma2(e, g[c * P + j], sb);
+            const int i = c * P + j;
+            if (VECTOR) dd[k][i] = dv[j];
+            const F2 q = mul2(dv[j], add2(xv[j], neg));
+            s1[i] = add2(s1[i], dv[j]);
+            s2[i] = fma2(q, r2, s2[i]);
+            sa = fma2(dv[j], g[i], sa);
+            sb = fma2(q, g[i], sb);
           }
         }
       sums[2 * k] = sum2(sa);
-      sums[2 * k + 1] = sum2(sb);
+      sums[2 * k + 1] = sum2(sb) * rstd[k];
     }
     const float mine = warp_sums<2 * R>(sums);
     if ((lane & 7) == 0) red[s & 1][warp][lane >> 3] = mine;
-    if (!__syncthreads_and(ok)) break;
-    // every thread is past the second pass of step s - 1
-    if (s > 0 && filled < steps) {
-      if (t == 0) fill(filled, freed);
-      if (++freed == p.stages) freed = 0;
-      ++filled;
-    }
+    if (!__syncthreads_and(ok)) return;
     if (a.dx != nullptr) {
       // lanes 8 v .. 8 v + 7 add value v's warp sums, then hand the total round
       float v = (lane & 7) < nw ? red[s & 1][lane & 7][lane >> 3] : 0.0f;
@@ -735,28 +734,31 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
       for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        const float ma = -__shfl_sync(0xffffffffu, v, 16 * k) * inv_d * rstd[k];
-        const float mb = -__shfl_sync(0xffffffffu, v, 16 * k + 8) * inv_d * rstd[k];
+        // dx = rstd (d g - A - z B) = (d g) rstd + (x c1 + c0)
+        const float ma = __shfl_sync(0xffffffffu, v, 16 * k) * inv_d;
+        const float mb = __shfl_sync(0xffffffffu, v, 16 * k + 8) * inv_d;
         if (k >= rows) continue;
-        const F2 neg = f2(-mean[k], -mean[k]), r2 = f2(rstd[k], rstd[k]);
-        const F2 ma2 = f2(ma, ma), mb2 = f2(mb, mb);
+        const float c1 = -rstd[k] * rstd[k] * mb, c0 = -mean[k] * c1 - rstd[k] * ma;
+        const F2 r2 = f2(rstd[k], rstd[k]), c12 = f2(c1, c1), c02 = f2(c0, c0);
         T* dx = static_cast<T*>(a.dx) + (base + s * R + k) * a.D;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           if (VECTOR && t + c * lanes >= nvec) continue;
-          F2 z[P], d[P];
-          values(src + 2 * k * p.x_slot, xl[k], dl[k], neg, r2, c, z, d);
+          F2 d[P], dv[P];
+          read(src + 2 * k * p.x_slot, xl[k], c, 0.0f, d);
+          if (!VECTOR) read(src + (2 * k + 1) * p.x_slot, dl[k], c, 0.0f, dv);
 #pragma unroll
           for (int j = 0; j < P; ++j)
-            d[j] = fma2(z[j], mb2, fma2(mul2(d[j], g[c * P + j]), r2, ma2));
+            d[j] = fma2(mul2(VECTOR ? dd[k][c * P + j] : dv[j], g[c * P + j]), r2,
+                        fma2(d[j], c12, c02));
           if constexpr (VECTOR) {
             *reinterpret_cast<uint4*>(dx + (t + c * lanes) * VEC) = repack<T>(d);
           } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-              const int col = t + (c * VEC + j) * lanes;
+              const int col = col0 + 32 * (c * VEC + j);
               const float2 f = split(d[j / 2]);
-              if (col < a.D) dx[col] = from_f32<T>(j & 1 ? f.y : f.x);
+              if (whole || col < a.D) dx[col] = from_f32<T>(j & 1 ? f.y : f.x);
             }
           }
         }
@@ -764,16 +766,11 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
     }
     if (++slot == p.stages) { slot = 0; phase ^= 1; }
   }
-  if (s < steps) {
-    if (t == 0) drain(full, p.stages, s, filled);
-    __syncthreads();
-    return;
-  }
   if (a.partial == nullptr) return;
   float* out = a.partial + (int64_t)blockIdx.x * 2 * a.D;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const int col = VECTOR ? (t + i / VEC * lanes) * VEC + i % VEC : t + i * lanes;
+    const int col = VECTOR ? (t + i / VEC * lanes) * VEC + i % VEC : col0 + 32 * i;
     const float2 u = split(s1[i / 2]), v = split(s2[i / 2]);
     if (col < a.D) {
       out[col] = i & 1 ? u.y : u.x;
@@ -993,7 +990,7 @@ int backward_staged_e(const BwdArgs& a, int64_t blocks, int64_t rows, int th, cu
   auto kern = backward_staged_kernel<T, E, VECTOR>;
   // the CTAs that the register file holds share the shared memory: three
   // slots at least (one read, one being freed, one in flight)
-  const int per_sm = std::max(1, std::min(8, 65536 / (th * (E <= 8 ? 80 : 128))));
+  const int per_sm = std::max(1, std::min(8, 65536 / ((th + 32) * (E <= 8 ? 72 : 128))));
   BwdPlan p;
   p.x_slot = (uint32_t)(a.D * (int)sizeof(T) + 15 + 15) / 16 * 16;
   p.last = rows - 1;
@@ -1004,19 +1001,21 @@ int backward_staged_e(const BwdArgs& a, int64_t blocks, int64_t rows, int th, cu
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
     return GWB_E_LAUNCH;
-  kern<<<(unsigned)blocks, th, smem, st>>>(a, p);
+  kern<<<(unsigned)blocks, th + 32, smem, st>>>(a, p);
   return launch_status();
 }
 
-// Eight columns a thread up to 384 threads, then sixteen; rows whose three
-// slots pass the shared memory take the wide form.
+// Eight columns a thread up to 384 threads, sixteen up to 480, then 24 (the
+// register file's shares); rows whose three slots pass the shared memory take the wide form.
 inline bool staged_fits(int D, int size) { return D <= 8192 && 3 * 4 * (D * size + 30) <= 226 * 1024; }
 template <typename T, bool VECTOR>
 int backward_staged(const BwdArgs& a, int64_t blocks, int64_t rows, cudaStream_t st) {
   const int unit = (a.D + 7) / 8;
   if (unit <= 384)
     return backward_staged_e<T, 8, VECTOR>(a, blocks, rows, (unit + 31) / 32 * 32, st);
-  return backward_staged_e<T, 16, VECTOR>(a, blocks, rows, ((a.D + 15) / 16 + 31) / 32 * 32, st);
+  if (unit <= 2 * 480)
+    return backward_staged_e<T, 16, VECTOR>(a, blocks, rows, ((a.D + 15) / 16 + 31) / 32 * 32, st);
+  return backward_staged_e<T, 24, VECTOR>(a, blocks, rows, ((a.D + 23) / 24 + 31) / 32 * 32, st);
 }
 
 template <typename T, int VEC>
