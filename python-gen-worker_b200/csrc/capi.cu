@@ -478,7 +478,7 @@ int gwb_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64
                       heads(k, k_strides, k_out, k_out_strides, k_heads), positions,
                       position_kind, position_strides[0], position_strides[1],
                       position_strides[2], inv_freq, axis, (int)axes, B * S_, (int)S_, (int)n,
-                      (int)head_dim, scale, inverse != 0, in_place, 1, 1};
+                      (int)head_dim, scale, inverse != 0, in_place};
   return gwb::launch_rotary(a, interleaved != 0, dtype, S(stream));
 }
 

@@ -34,6 +34,8 @@ template <typename T, int VEC> struct Pack {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
   __device__ __forceinline__ float get(int j) const { return to_f32<T>(raw.v[j]); }
   __device__ __forceinline__ void set(int j, float f) { raw.v[j] = from_f32<T>(f); }
+  __device__ __forceinline__ uint4 bits() const { return *reinterpret_cast<const uint4*>(&raw); }
+  __device__ __forceinline__ void put(uint4 w) { *reinterpret_cast<uint4*>(&raw) = w; }
 };
 
 // Two f32 in one 64-bit register: sm_100 multiplies and adds both in one

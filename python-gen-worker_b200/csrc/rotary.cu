@@ -18,6 +18,20 @@
 namespace gwb {
 namespace rotary {
 
+// Division of n < 2^31 by a fixed d as a multiply and a shift.
+struct FastDiv {
+  uint32_t d, m, s;
+  __host__ static FastDiv of(uint32_t d) {
+    FastDiv f{d, 0, 0};
+    while ((1ull << f.s) < d) ++f.s;                 // ceil(log2 d)
+    f.m = (uint32_t)(((1ull << 32) * ((1ull << f.s) - d)) / d + 1);
+    return f;
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return (uint32_t)(((uint64_t)__umulhi(n, m) + n) >> s);
+  }
+};
+
 struct Heads {                     // q or k: [B, S, H, Dh] by strides, last dim dense
   const void* x; void* y;
   int64_t xb, xs, xh, yb, ys, yh;  // element strides
@@ -34,8 +48,11 @@ struct Args {
   int64_t tokens; int S;           // B * S, S
   int n, dh;                       // rotated pairs, head size
   float scale; int inverse, in_place;
-  int split;                       // CTAs that share a token's heads
-  int per_cta;                     // tokens a CTA takes
+  int64_t total;                   // units of all tokens
+  int chunk;                       // units a CTA takes
+  int items, rot_items;            // of a head
+  int per_thread;                  // heads a thread
+  FastDiv by_token, by_item, by_seq, by_n;   // units of a token, items, S, n
 };
 
 constexpr double kInvTwoPi = 0.15915494309189533576888;
@@ -47,81 +64,134 @@ __device__ __forceinline__ double position_of(const Args& a, int64_t b, int64_t 
   return (double)static_cast<const float*>(a.pos)[at];
 }
 
-// Threads (x, y): x walks one head's items, y the heads. An item is one
-// vector of pairs (two 16-byte accesses in the half layout, one interleaved)
-// or, out of place, one vector of the features that pass through.
+// The rotation, with its roundings in one order in every form, so that a
+// tensor's alignment does not change its bits.
+__device__ __forceinline__ float first_of(float p, float r, float c, float s) {
+  return fmaf(r, -s, __fmul_rn(p, c));
+}
+__device__ __forceinline__ float second_of(float p, float r, float c, float s) {
+  return fmaf(p, s, __fmul_rn(r, c));
+}
+
+// An item is one vector of pairs (two 16-byte accesses in the half layout,
+// one interleaved) or, out of place, one vector of the features that pass
+// through. A thread takes one item of up to HEADS consecutive heads of a
+// token: the indices and the item's cosines and sines are worked out once for
+// all of them, and their loads are in flight together. A CTA takes a run of
+// consecutive units (token, group of heads, item), so sizes that divide by
+// nothing leave no thread idle; its loads are in flight while it works out
+// the angles. (An item and head a thread spent more
+// instructions on indices than on the rotation: 41 us against 25 at 4608
+// tokens of 48 heads.)
+constexpr int THREADS = 256;
+// heads a thread: 32 registers of loads in flight, or eight elements
+template <int VEC, bool INTERLEAVED> constexpr int heads_of() {
+  return INTERLEAVED && VEC > 1 ? 8 : 4;
+}
+
 template <typename T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rotary_kernel(const Args a) {
-  extern __shared__ float2 turn[];             // [per_cta][n] (c cos, c sin)
-  const int tid = threadIdx.y * blockDim.x + threadIdx.x, nthreads = blockDim.x * blockDim.y;
-  const int64_t t0 = (int64_t)(blockIdx.x / a.split) * a.per_cta;
-  const int part = blockIdx.x % a.split;
-  const int nt = (int)(a.tokens - t0 < a.per_cta ? a.tokens - t0 : a.per_cta);
-  for (int i = tid; i < nt * a.n; i += nthreads) {
-    const int64_t tok = t0 + i / a.n;
-    const int f = i % a.n;
+__global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const Args a) {
+  extern __shared__ __align__(16) float turn[];          // [tokens of the run][2][n] c cos, c sin
+  constexpr bool ONE = INTERLEAVED && VEC > 1;           // one access an item
+  constexpr int PAIRS = ONE ? VEC / 2 : VEC;             // pairs an item
+  constexpr int HEADS = heads_of<VEC, INTERLEAVED>();
+  const int64_t u0 = (int64_t)blockIdx.x * a.chunk;
+  const int count = (int)(a.total - u0 < a.chunk ? a.total - u0 : a.chunk);
+  const uint32_t tok0 = (uint32_t)(u0 / a.by_token.d), lead = (uint32_t)(u0 % a.by_token.d);
+  const uint32_t n = lead + threadIdx.x, k = a.by_token.div(n), rem = n - k * a.by_token.d;
+  const uint32_t grp = a.by_item.div(rem);
+  const int item = (int)(rem - grp * a.by_item.d);
+  const uint32_t tok = tok0 + k, b = a.by_seq.div(tok), s = tok - b * a.by_seq.d;
+  const int h0 = (int)grp * a.per_thread;
+  const int hn = (int)threadIdx.x < count ? min(a.per_thread, a.q.h + a.k.h - h0) : 0;
+  const bool rot = item < a.rot_items;
+  // offset of the item's first vector, and of its second from there
+  const int ia = rot ? (ONE ? item * VEC : INTERLEAVED ? 2 * item : item * VEC)
+                     : 2 * a.n + (item - a.rot_items) * VEC;
+  const int gap = INTERLEAVED ? 1 : a.n;
+  Pack<T, VEC> va[HEADS], vb[ONE ? 1 : HEADS];
+  {
+    const T* qx = static_cast<const T*>(a.q.x) + b * a.q.xb + s * a.q.xs + ia;
+    const T* kx = static_cast<const T*>(a.k.x) + b * a.k.xb + s * a.k.xs + ia;
+#pragma unroll
+    for (int j = 0; j < HEADS; ++j)
+      if (j < hn) {
+        const int h = h0 + j;
+        const T* x = h < a.q.h ? qx + h * a.q.xh : kx + (h - a.q.h) * a.k.xh;
+        va[j].load(x);
+        if constexpr (!ONE) if (rot) vb[j].load(x + gap);
+      }
+  }
+  // the angles, while the loads are in flight
+  const int nt = (int)a.by_token.div(lead + count - 1) + 1;
+  for (int i = threadIdx.x; i < nt * a.n; i += THREADS) {
+    const uint32_t kk = a.by_n.div(i), f = i - kk * a.n, tk = tok0 + kk;
+    const uint32_t bb = a.by_seq.div(tk), ss = tk - bb * a.by_seq.d;
     int ax = a.axis ? a.axis[f] : 0;
     ax = ax < 0 ? 0 : ax >= a.axes ? a.axes - 1 : ax;   // a bad axis reads no stray position
-    const double p = position_of(a, tok / a.S, tok % a.S, ax);
-    const double turns = p * a.inv_freq[f] * kInvTwoPi;
+    const double turns = position_of(a, bb, ss, ax) * a.inv_freq[f] * kInvTwoPi;
     const float frac = (float)(turns - rint(turns));
     float sn, cs;
     sincospif(2.0f * frac, &sn, &cs);
-    turn[i] = make_float2(cs * a.scale, (a.inverse ? -sn : sn) * a.scale);
+    turn[2 * kk * a.n + f] = cs * a.scale;
+    turn[(2 * kk + 1) * a.n + f] = (a.inverse ? -sn : sn) * a.scale;
   }
   __syncthreads();
-  // items: rotated vectors, then (out of place) pass-through vectors
-  constexpr int PAIRS = INTERLEAVED && VEC > 1 ? VEC / 2 : VEC;   // pairs an item
-  const int rot_items = a.n / PAIRS;
-  const int rest = a.dh - 2 * a.n;
-  const int items = rot_items + (a.in_place ? 0 : rest / VEC);
-  const int heads = a.q.h + a.k.h;
-  for (int k = 0; k < nt; ++k) {
-    const int64_t tok = t0 + k, b = tok / a.S, s = tok % a.S;
-    const float2* tr = turn + k * a.n;
-    for (int h = part * blockDim.y + threadIdx.y; h < heads; h += blockDim.y * a.split) {
-      const bool is_k = h >= a.q.h;
-      const Heads& w = is_k ? a.k : a.q;
-      const int hh = is_k ? h - a.q.h : h;
-      const T* x = static_cast<const T*>(w.x) + b * w.xb + s * w.xs + hh * w.xh;
-      T* y = static_cast<T*>(w.y) + b * w.yb + s * w.ys + hh * w.yh;
-      for (int i = threadIdx.x; i < items; i += blockDim.x) {
-        if (i < rot_items) {
-          if constexpr (INTERLEAVED && VEC > 1) {
-            Pack<T, VEC> v;
-            v.load(x + i * VEC);
+  float c[PAIRS], sn[PAIRS];
+  if (rot && hn > 0) {
+    const float* tr = turn + 2 * k * a.n + item * PAIRS;
+    if constexpr (PAIRS % 4 == 0) {
 #pragma unroll
-            for (int j = 0; j < VEC; j += 2) {
-              const float2 c = tr[i * PAIRS + j / 2];
-              const float p = v.get(j), r = v.get(j + 1);
-              v.set(j, p * c.x - r * c.y);
-              v.set(j + 1, r * c.x + p * c.y);
-            }
-            v.store(y + i * VEC);
-          } else {
-            const int ia = INTERLEAVED ? 2 * i : i * VEC, ib = INTERLEAVED ? ia + 1 : a.n + ia;
-            Pack<T, VEC> va, vb;
-            va.load(x + ia);
-            vb.load(x + ib);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              const float2 c = tr[i * VEC + j];
-              const float p = va.get(j), r = vb.get(j);
-              va.set(j, p * c.x - r * c.y);
-              vb.set(j, r * c.x + p * c.y);
-            }
-            va.store(y + ia);
-            vb.store(y + ib);
-          }
-        } else {
-          const int at = 2 * a.n + (i - rot_items) * VEC;
-          Pack<T, VEC> v;
-          v.load(x + at);
-          v.store(y + at);
-        }
+      for (int e = 0; e < PAIRS; e += 4) {
+        *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(tr + e);
+        *reinterpret_cast<float4*>(sn + e) = *reinterpret_cast<const float4*>(tr + a.n + e);
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) { c[e] = tr[e]; sn[e] = tr[a.n + e]; }
     }
   }
+  T* qy = static_cast<T*>(a.q.y) + b * a.q.yb + s * a.q.ys + ia;
+  T* ky = static_cast<T*>(a.k.y) + b * a.k.yb + s * a.k.ys + ia;
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j)
+    if (j < hn) {
+      const int h = h0 + j;
+      T* y = h < a.q.h ? qy + h * a.q.yh : ky + (h - a.q.h) * a.k.yh;
+      if (rot) {
+        if constexpr (VEC == 1) {
+          const float p = va[j].get(0), r = vb[j].get(0);
+          va[j].set(0, first_of(p, r, c[0], sn[0]));
+          vb[j].set(0, second_of(p, r, c[0], sn[0]));
+          vb[j].store(y + gap);
+        } else if constexpr (ONE) {
+          F2 v[PAIRS];
+          unpack<T>(va[j].bits(), v);
+#pragma unroll
+          for (int e = 0; e < PAIRS; ++e) {
+            const float2 f = split(v[e]);
+            v[e] = f2(first_of(f.x, f.y, c[e], sn[e]), second_of(f.x, f.y, c[e], sn[e]));
+          }
+          va[j].put(repack<T>(v));
+        } else {
+          F2 p[PAIRS / 2], r[PAIRS / 2];
+          unpack<T>(va[j].bits(), p);
+          unpack<T>(vb[j].bits(), r);
+#pragma unroll
+          for (int e = 0; e < PAIRS / 2; ++e) {
+            const F2 c2 = f2(c[2 * e], c[2 * e + 1]), s2 = f2(sn[2 * e], sn[2 * e + 1]);
+            const F2 n2 = f2(-sn[2 * e], -sn[2 * e + 1]);
+            const F2 u = fma2(r[e], n2, mul2(p[e], c2));
+            r[e] = fma2(p[e], s2, mul2(r[e], c2));
+            p[e] = u;
+          }
+          va[j].put(repack<T>(p));
+          vb[j].put(repack<T>(r));
+          vb[j].store(y + gap);
+        }
+      }
+      va[j].store(y);
+    }
 }
 
 inline bool vec_heads(const Heads& w, int V) {
@@ -134,32 +204,29 @@ inline bool vec_heads(const Heads& w, int V) {
 template <typename T, int VEC, bool INTERLEAVED>
 int launch_v(Args a, cudaStream_t st) {
   constexpr int PAIRS = INTERLEAVED && VEC > 1 ? VEC / 2 : VEC;
-  const int items = a.n / PAIRS + (a.in_place ? 0 : (a.dh - 2 * a.n) / VEC);
+  a.rot_items = a.n / PAIRS;
+  a.items = a.rot_items + (a.in_place ? 0 : (a.dh - 2 * a.n) / VEC);
   const int heads = a.q.h + a.k.h;
-  const int bx = items < 256 ? (items > 0 ? items : 1) : 256;
-  int by = 256 / bx;
-  if (by > heads) by = heads;
-  // With few tokens a token's heads are split over CTAs until the GPU has two
-  // CTAs a multiprocessor (each repeats the token's angles, n of them); with
-  // many, a CTA takes tokens until its threads have two items each, as far
-  // as the angles fit.
-  a.split = 1;
-  a.per_cta = 1;
-  const int most_split = (heads + by - 1) / by;
-  if (a.tokens < 296) {
-    const int64_t want = (296 + a.tokens - 1) / a.tokens;
-    a.split = (int)(want < most_split ? want : most_split);
-  } else {
-    const int rows = (heads + by - 1) / by;
-    const int xs = (items + bx - 1) / bx;
-    while (a.per_cta < 8 && a.per_cta * rows * xs < 2 && a.tokens / (a.per_cta * 2) >= 148 * 8 &&
-           (a.per_cta * 2) * a.n <= 4096)
-      a.per_cta *= 2;
-  }
-  const int64_t blocks = (a.tokens + a.per_cta - 1) / a.per_cta * a.split;
+  // heads a thread: as many as still give every multiprocessor four CTAs
+  a.per_thread = heads_of<VEC, INTERLEAVED>();
+  while (a.per_thread > 1 &&
+         a.tokens * ((heads + a.per_thread - 1) / a.per_thread) * a.items < (int64_t)148 * 4 * THREADS)
+    a.per_thread /= 2;
+  const int64_t groups = (heads + a.per_thread - 1) / a.per_thread, per_token = groups * a.items;
+  if (per_token > 1 << 24) return GWB_E_CAPACITY;
+  a.total = a.tokens * per_token;
+  a.by_token = FastDiv::of((uint32_t)per_token);
+  a.by_item = FastDiv::of((uint32_t)a.items);
+  a.by_seq = FastDiv::of((uint32_t)a.S);
+  a.by_n = FastDiv::of((uint32_t)(a.n > 0 ? a.n : 1));
+  // units a CTA: one a thread, as many as the angles of their tokens fit in 48 KB
+  a.chunk = THREADS;
+  const auto tokens = [&](int chunk) { return (chunk + per_token - 2) / per_token + 1; };
+  while (a.chunk > 8 && tokens(a.chunk) * a.n * 2 * (int64_t)sizeof(float) > 48 * 1024) a.chunk /= 2;
+  const int64_t blocks = (a.total + a.chunk - 1) / a.chunk;
   if (blocks > 0x7fffffff) return GWB_E_CAPACITY;
-  const size_t smem = (size_t)a.per_cta * a.n * sizeof(float2);
-  rotary_kernel<T, VEC, INTERLEAVED><<<(unsigned)blocks, dim3(bx, by), smem, st>>>(a);
+  const size_t smem = (size_t)tokens(a.chunk) * a.n * 2 * sizeof(float);
+  rotary_kernel<T, VEC, INTERLEAVED><<<(unsigned)blocks, THREADS, smem, st>>>(a);
   return launch_status();
 }
 
