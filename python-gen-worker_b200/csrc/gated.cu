@@ -11,7 +11,7 @@
 // memory: the backward products read W, x and dg / du as they lie, through
 // MN-major shared-memory descriptors.
 //
-//   FORWARD  128 x (128 gate | 128 up) tile: both projections accumulate side
+//   FORWARD  256 x (128 gate | 128 up) tile: both projections accumulate side
 //            by side in TMEM, so activation and product happen in registers
 //            and g and u never reach memory.
 //   DGATE    the same tile again; the epilogue reads dh and writes dg and du
@@ -33,18 +33,21 @@ namespace gated {
 
 enum Mode { FORWARD, DGATE, DX, DW };
 
+// A pair of CTAs shares a 256 x 256 tile: each holds its 128 rows of A, half
+// of B's rows and its 128 rows of the accumulator, so a stage costs 32 KB a CTA
+// where a CTA alone needs 48 KB for a 128 x 256 tile, and a third less is
+// copied and read from shared memory per operation.
 constexpr int BM = 128, BN = 256, BK = 64;      // BK elements = one 128-byte swizzle row
-constexpr int STAGES = 4;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
+constexpr int STAGES = 6;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / 2 * BK * 2;   // of one CTA
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int MN_BOX = 64 * BK * 2;             // a 64 (MN) x 64 (K) box of an MN-major operand
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
 constexpr int THREADS = 384, EPI0 = 4, EPI_WARPS = 8;
 constexpr int NACC = 2, TMEM_COLS = NACC * BN;
-// Tiles are walked in groups of 16 row tiles: 148 tiles at once then read
-// about 16 row tiles and 9 column tiles (twice as wide), the least operand
-// bytes for a product of the two counts.
-constexpr int GROUP = 16;
+// Tiles are walked in groups of eight row tiles: the 74 pairs at work then read
+// about 8 row tiles and 9 column tiles, near the fewest operand bytes.
+constexpr int GROUP = 8;
 
 struct Args {
   const void* bg; const void* bu;     // FORWARD, DGATE: biases [F] or null
@@ -95,7 +98,7 @@ template <typename T, bool A_MN, bool B_MN>
 __host__ __device__ constexpr uint32_t idesc16() {
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
-         ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+         ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(2 * BM >> 4) << 24);
 }
 
 struct Tile { int m0, n0, half; };
@@ -106,10 +109,18 @@ __device__ __forceinline__ Tile tile_of(const Args& a, int t) {
   const int rows = min(a.tiles_m - first, GROUP), in = t % per;
   const int tm = first + in % rows, tn = in / rows;
   if (MODE == DW) {
-    const int tf = (a.F + BM - 1) / BM;
-    return {(tm % tf) * BM, tn * BN, a.half0 + tm / tf};
+    const int tf = (a.F + 2 * BM - 1) / (2 * BM);
+    return {(tm % tf) * 2 * BM, tn * BN, a.half0 + tm / tf};
   }
-  return {tm * BM, tn * (MODE == DX ? BN : BN / 2), 0};
+  return {tm * 2 * BM, tn * (MODE == DX ? BN : BN / 2), 0};
+}
+
+// After a wait that ran out: a millisecond, in which any copy in flight lands
+// before the CTA gives its shared memory back (the barrier that would tell is
+// the other CTA's).
+__device__ __forceinline__ void land_copies() {
+  const long long t = clock64();
+  while (clock64() - t < 2000000) { }
 }
 
 template <typename T, int N>
@@ -121,35 +132,40 @@ __device__ __forceinline__ void load8(const T* p, float (&f)[N]) {
 }
 
 template <int MODE, typename T>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
              const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1,
              const Args a) {
   constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);   // the leader's count
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
-  uint64_t* acc_empty = acc_full + NACC;
+  uint64_t* acc_empty = acc_full + NACC;                                       // the leader's count
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + NACC);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int kext = MODE == DX ? a.F : MODE == DW ? a.M : a.D;
   const int nk1 = (kext + BK - 1) / BK;               // k-blocks of one segment
   const int nk = MODE == DX ? 2 * nk1 : nk1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < NACC; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], EPI_WARPS); }
+    for (int i = 0; i < NACC; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * EPI_WARPS);
+    }
     fence_barrier_init();
     tma_prefetch_desc(&tA0);
     tma_prefetch_desc(&tB0);
     if (MODE != DW) tma_prefetch_desc(&tB1);
     if (B_MN) tma_prefetch_desc(&tA1);
   }
-  if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, TMEM_COLS);
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
@@ -160,8 +176,10 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
     if (warp == 0 && lane == 0) {
       int it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < a.ntiles; tile += gridDim.x) {
+      for (int tile = pair; ok && tile < a.ntiles; tile += pairs) {
         const Tile t = tile_of<MODE>(a, tile);
+        const int m0 = t.m0 + (int)rank * BM;         // this CTA's rows of A
+        const int bn = (int)rank * (BN / 2);          // its part of B's rows
         for (int kb = 0; kb < nk; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, GWB_ERR_TIMEOUT_PRODUCER)) {
@@ -170,33 +188,38 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
           }
           uint8_t* sa = smem + s * STAGE_BYTES;
           uint8_t* sb = sa + A_BYTES;
-          mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
+          // both CTAs' copies complete on the leader's barrier, which expects
+          // them all; the other CTA's may come first, the phase still waits
+          // for the leader's arrival
+          const uint32_t bar = cluster_addr(&full[s], 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
           if constexpr (MODE == FORWARD || MODE == DGATE) {
-            tma_load_2d(sa, &tA0, &full[s], kb * BK, t.m0);
-            tma_load_2d(sb, &tB0, &full[s], kb * BK, t.n0);
-            tma_load_2d(sb + B_BYTES / 2, &tB1, &full[s], kb * BK, t.n0);
+            // the pair's 256 rows of B: the leader's are the gate's, the other's the up's
+            tma_load_2d_pair(sa, &tA0, bar, kb * BK, m0);
+            tma_load_2d_pair(sb, rank ? &tB1 : &tB0, bar, kb * BK, t.n0);
           } else if constexpr (MODE == DX) {
             const bool up = kb >= nk1;
             const int k0 = (kb - (up ? nk1 : 0)) * BK;
-            tma_load_2d(sa, up ? &tA1 : &tA0, &full[s], k0, t.m0);
+            tma_load_2d_pair(sa, up ? &tA1 : &tA0, bar, k0, m0);
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j)
-              tma_load_2d(sb + j * MN_BOX, up ? &tB1 : &tB0, &full[s], t.n0 + 64 * j, k0);
+            for (int j = 0; j < BN / 128; ++j)
+              tma_load_2d_pair(sb + j * MN_BOX, up ? &tB1 : &tB0, bar, t.n0 + bn + 64 * j, k0);
           } else {
 #pragma unroll
             for (int j = 0; j < BM / 64; ++j)
-              tma_load_2d(sa + j * MN_BOX, t.half ? &tA1 : &tA0, &full[s], t.m0 + 64 * j, kb * BK);
+              tma_load_2d_pair(sa + j * MN_BOX, t.half ? &tA1 : &tA0, bar, m0 + 64 * j, kb * BK);
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j)
-              tma_load_2d(sb + j * MN_BOX, &tB0, &full[s], t.n0 + 64 * j, kb * BK);
+            for (int j = 0; j < BN / 128; ++j)
+              tma_load_2d_pair(sb + j * MN_BOX, &tB0, bar, t.n0 + bn + 64 * j, kb * BK);
           }
         }
       }
-    } else if (warp == 1 && lane == 0) {
+      if (!ok) land_copies();
+    } else if (warp == 1 && lane == 0 && rank == 0) {
       constexpr uint32_t idesc = idesc16<T, A_MN, B_MN>();
       int it = 0, lt = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < a.ntiles; tile += gridDim.x, ++lt) {
+      for (int tile = pair; ok && tile < a.ntiles; tile += pairs, ++lt) {
         const int b = lt & 1;
         if (!mbar_wait(&acc_empty[b], ((lt >> 1) & 1) ^ 1, GWB_ERR_TIMEOUT_MMA)) break;
         tc_fence_after();
@@ -208,20 +231,21 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
           const uint32_t ab = smem_u32(smem + s * STAGE_BYTES), bb = ab + A_BYTES;
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_f16(d, A_MN ? sdesc_mn128(ab + 2048 * k, MN_BOX) : sdesc_k128(ab + 32 * k),
-                    B_MN ? sdesc_mn128(bb + 2048 * k, MN_BOX) : sdesc_k128(bb + 32 * k), idesc,
-                    (kb > 0 || k > 0) ? 1u : 0u);
-          mma_commit(&empty[s]);
+            mma_f16_pair(d, A_MN ? sdesc_mn128(ab + 2048 * k, MN_BOX) : sdesc_k128(ab + 32 * k),
+                         B_MN ? sdesc_mn128(bb + 2048 * k, MN_BOX) : sdesc_k128(bb + 32 * k), idesc,
+                         (kb > 0 || k > 0) ? 1u : 0u);
+          mma_commit_pair(&empty[s]);
         }
-        if (ok) mma_commit(&acc_full[b]);
+        if (ok) mma_commit_pair(&acc_full[b]);
       }
     }
   } else {
     regs_inc<232>();
     const int q = warp & 3, side = (warp - EPI0) >> 2;
     int lt = 0;
-    for (int tile = blockIdx.x; tile < a.ntiles; tile += gridDim.x, ++lt) {
-      const Tile t = tile_of<MODE>(a, tile);
+    for (int tile = pair; tile < a.ntiles; tile += pairs, ++lt) {
+      Tile t = tile_of<MODE>(a, tile);
+      t.m0 += (int)rank * BM;
       const int b = lt & 1;
       if (!mbar_wait(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
       __syncwarp();
@@ -242,7 +266,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[b]);
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[b], 0));
       if constexpr (MODE == FORWARD || MODE == DGATE) {
         if (row >= a.M) continue;
         const int n0 = t.n0 + 64 * side;
@@ -298,9 +322,11 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
       }
     }
   }
+  // neither CTA ends while the other's MMAs, arrivals or copies may reach it
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
+  cluster_sync();
+  if (warp == 1) tmem_dealloc_pair(tmem, TMEM_COLS);
 }
 
 // ------------------------------------------------------------- bias gradients
@@ -378,8 +404,8 @@ int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0,
       return GWB_E_LAUNCH;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int n_sm = sm_count();
-  kern<<<a.ntiles < n_sm ? a.ntiles : n_sm, THREADS, SMEM_BYTES, st>>>(a0, a1, b0, b1, a);
+  const int pairs = sm_count() / 2;
+  kern<<<2 * (a.ntiles < pairs ? a.ntiles : pairs), THREADS, SMEM_BYTES, st>>>(a0, a1, b0, b1, a);
   return launch_status();
 }
 
@@ -403,7 +429,7 @@ int projections(bool dgate, const void* x, int64_t xs, const void* wg, const voi
   if (int rc = tmap16(&tx, x, bf, a.D, a.M, xs, BM)) return rc;
   if (int rc = tmap16(&tg, wg, bf, a.D, a.F, a.D, BN / 2)) return rc;
   if (int rc = tmap16(&tu, wu, bf, a.D, a.F, a.D, BN / 2)) return rc;
-  a.tiles_m = cdiv(a.M, BM);
+  a.tiles_m = cdiv(a.M, 2 * BM);
   a.tiles_n = cdiv(a.F, BN / 2);
   a.ntiles = a.tiles_m * a.tiles_n;
   return dgate ? launch<DGATE, T>(tx, tx, tg, tu, a, st) : launch<FORWARD, T>(tx, tx, tg, tu, a, st);
@@ -437,7 +463,7 @@ int backward(const GatedBackward& w, cudaStream_t st) {
     if (int rc = tmap16(&bum, w.wu, bf, D, F, D, BK)) return rc;
     Args c = a;
     c.o0 = w.dx;
-    c.tiles_m = cdiv(M, BM);
+    c.tiles_m = cdiv(M, 2 * BM);
     c.tiles_n = cdiv(D, BN);
     c.ntiles = c.tiles_m * c.tiles_n;
     if (int rc = launch<DX, T>(ag, au, bgm, bum, c, st)) return rc;
@@ -451,7 +477,7 @@ int backward(const GatedBackward& w, cudaStream_t st) {
     c.o0 = w.dwg;
     c.o1 = w.dwu;
     c.half0 = w.dwg ? 0 : 1;
-    c.tiles_m = cdiv(F, BM) * (w.dwg && w.dwu ? 2 : 1);
+    c.tiles_m = cdiv(F, 2 * BM) * (w.dwg && w.dwu ? 2 : 1);
     c.tiles_n = cdiv(D, BN);
     c.ntiles = c.tiles_m * c.tiles_n;
     if (int rc = launch<DW, T>(ag, au, bx, bx, c, st)) return rc;
