@@ -373,20 +373,30 @@ int gwb_gated_linear(const void* x, int64_t x_stride, const void* w_gate, const 
                      const void* b_gate, const void* b_up, int64_t M, int64_t D, int64_t F,
                      int activation, int dtype, void* h, void* stream);
 
+/* gwb_gated_linear for a backward pass to come: also writes `kept`
+ * (gwb_gated_linear_kept bytes, 16-byte aligned), what the backward call
+ * needs of the projections: u act'(g) and act(g), 4 bytes a pair for bf16 (as
+ * f16 with a power of two per row and 64 columns), 8 for f16 (as f32). */
+int gwb_gated_linear_keep(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
+                          const void* b_gate, const void* b_up, int64_t M, int64_t D, int64_t F,
+                          int activation, int dtype, void* h, void* kept, void* stream);
+int64_t gwb_gated_linear_kept(int64_t M, int64_t F, int dtype);
+
 /* Bytes of the 256-byte aligned scratch `work` of gwb_gated_linear_backward
  * (0 when a size is not positive). */
 int64_t gwb_gated_linear_backward_work(int64_t M, int64_t F);
 
 /* Gradients of gwb_gated_linear, each NULL when not wanted: dx [M, D],
  * dw_gate / dw_up [F, D], db_gate / db_up [F], from dh [M, F] (row stride
- * dh_stride). The projections are computed again rather than kept from the
- * forward call; dg and du are rounded to `dtype` as the operands of the
- * gradients' products. No atomics: the same call gives the same bits. */
+ * dh_stride). `kept` from gwb_gated_linear_keep on the same arguments, or NULL:
+ * the projections are then computed again. dg and du are rounded to `dtype`
+ * as the operands of the gradients' products. No atomics: the same call gives
+ * the same bits. */
 int gwb_gated_linear_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
                               const void* w_gate, const void* w_up, const void* b_gate,
-                              const void* b_up, int64_t M, int64_t D, int64_t F, int activation,
-                              int dtype, void* dx, void* dw_gate, void* dw_up, void* db_gate,
-                              void* db_up, void* work, void* stream);
+                              const void* b_up, void* kept, int64_t M, int64_t D, int64_t F,
+                              int activation, int dtype, void* dx, void* dw_gate, void* dw_up,
+                              void* db_gate, void* db_up, void* work, void* stream);
 
 /* Reads and clears the device-side error flag set by a bounded wait that
  * expired (0 = none; 1 TMA producer, 2 MMA thread, 3 epilogue, 4 unpack

@@ -492,18 +492,37 @@ static int gated_sizes(int64_t M, int64_t D, int64_t F, int activation, int dtyp
   return dtype == GWB_BF16 || dtype == GWB_F16 ? GWB_SUCCESS : GWB_E_SHAPE;
 }
 
+static int gated_call(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
+                      const void* b_gate, const void* b_up, int64_t M, int64_t D, int64_t F,
+                      int activation, int dtype, void* h, bool keep, void* kept, void* stream) {
+  if (int rc = gated_sizes(M, D, F, activation, dtype)) return rc;
+  if (M == 0) return GWB_SUCCESS;
+  if (!x || !w_gate || !w_up || !h || (keep && !kept)) return GWB_E_SHAPE;
+  if (x_stride < D || x_stride % 8) return GWB_E_SHAPE;
+  if (!al16(x) || !al16(w_gate) || !al16(w_up) || !al16(h) || (b_gate && !al16(b_gate)) ||
+      (b_up && !al16(b_up)) || !al16(kept))
+    return GWB_E_ALIGN;
+  return gwb::launch_gated_forward(x, x_stride, w_gate, w_up, b_gate, b_up, (int)M, (int)D, (int)F,
+                                   activation, dtype, h, keep ? kept : nullptr, S(stream));
+}
+
 int gwb_gated_linear(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
                      const void* b_gate, const void* b_up, int64_t M, int64_t D, int64_t F,
                      int activation, int dtype, void* h, void* stream) {
-  if (int rc = gated_sizes(M, D, F, activation, dtype)) return rc;
-  if (M == 0) return GWB_SUCCESS;
-  if (!x || !w_gate || !w_up || !h) return GWB_E_SHAPE;
-  if (x_stride < D || x_stride % 8) return GWB_E_SHAPE;
-  if (!al16(x) || !al16(w_gate) || !al16(w_up) || !al16(h) || (b_gate && !al16(b_gate)) ||
-      (b_up && !al16(b_up)))
-    return GWB_E_ALIGN;
-  return gwb::launch_gated_forward(x, x_stride, w_gate, w_up, b_gate, b_up, (int)M, (int)D, (int)F,
-                                   activation, dtype, h, S(stream));
+  return gated_call(x, x_stride, w_gate, w_up, b_gate, b_up, M, D, F, activation, dtype, h, false,
+                    nullptr, stream);
+}
+
+int gwb_gated_linear_keep(const void* x, int64_t x_stride, const void* w_gate, const void* w_up,
+                          const void* b_gate, const void* b_up, int64_t M, int64_t D, int64_t F,
+                          int activation, int dtype, void* h, void* kept, void* stream) {
+  return gated_call(x, x_stride, w_gate, w_up, b_gate, b_up, M, D, F, activation, dtype, h, true,
+                    kept, stream);
+}
+
+int64_t gwb_gated_linear_kept(int64_t M, int64_t F, int dtype) {
+  if (!fits_int(M) || !fits_int(F) || M == 0 || F == 0) return 0;
+  return dtype == GWB_BF16 || dtype == GWB_F16 ? gwb::gated_kept_bytes(M, F, dtype) : 0;
 }
 
 int64_t gwb_gated_linear_backward_work(int64_t M, int64_t F) {
@@ -513,9 +532,9 @@ int64_t gwb_gated_linear_backward_work(int64_t M, int64_t F) {
 
 int gwb_gated_linear_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
                               const void* w_gate, const void* w_up, const void* b_gate,
-                              const void* b_up, int64_t M, int64_t D, int64_t F, int activation,
-                              int dtype, void* dx, void* dw_gate, void* dw_up, void* db_gate,
-                              void* db_up, void* work, void* stream) {
+                              const void* b_up, void* kept, int64_t M, int64_t D, int64_t F,
+                              int activation, int dtype, void* dx, void* dw_gate, void* dw_up,
+                              void* db_gate, void* db_up, void* work, void* stream) {
   if (int rc = gated_sizes(M, D, F, activation, dtype)) return rc;
   if (M == 0) {
     // no rows: the parameters' gradients are zero
@@ -529,11 +548,11 @@ int gwb_gated_linear_backward(const void* dh, int64_t dh_stride, const void* x, 
   if (!dh || !x || !w_gate || !w_up || !work) return GWB_E_SHAPE;
   if (x_stride < D || x_stride % 8 || dh_stride < F || dh_stride % 8) return GWB_E_SHAPE;
   for (const void* p : {dh, x, w_gate, w_up, b_gate, b_up, (const void*)dx, (const void*)dw_gate,
-                        (const void*)dw_up, (const void*)work})
+                        (const void*)dw_up, (const void*)kept, (const void*)work})
     if (!al16(p)) return GWB_E_ALIGN;
   if (!dx && !dw_gate && !dw_up && !db_gate && !db_up) return GWB_SUCCESS;
   gwb::GatedBackward w{dh, dh_stride, x, x_stride, w_gate, w_up, b_gate, b_up, (int)M, (int)D,
-                       (int)F, activation, dx, dw_gate, dw_up, db_gate, db_up, work};
+                       (int)F, activation, dx, dw_gate, dw_up, db_gate, db_up, kept, work};
   return gwb::launch_gated_backward(w, dtype, S(stream));
 }
 

@@ -14,13 +14,19 @@
 //   FORWARD  256 x (128 gate | 128 up) tile: both projections accumulate side
 //            by side in TMEM, so activation and product happen in registers
 //            and g and u never reach memory.
-//   DGATE    the same tile again; the epilogue reads dh and writes dg and du
-//            (rounded to the operand type: they are tensor-core operands next).
+//   SAVE     FORWARD for a backward pass to come: also writes a = u act'(g) and
+//            b = act(g), all that dg = dh a and du = dh b need of it.
+//   DGATE    the same tile again for a caller that kept nothing; the epilogue
+//            reads dh and writes dg and du (rounded to the operand type: they
+//            are tensor-core operands next).
 //   DX       dg Wg + du Wu as one chain of K = 2 F into one accumulator.
 //   DW       dg^T x and du^T x, K = M.
 //
 // Accumulators, activations and column sums are f32; every output is rounded
-// once.
+// once. a and b are kept with three bits or more beyond the operand type's, so
+// that keeping them adds next to nothing to the rounding of dg and du: for bf16
+// as f16 times a power of two per row and 64 columns (4 bytes a pair), for f16
+// as f32.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <atomic>
@@ -31,7 +37,7 @@
 namespace gwb {
 namespace gated {
 
-enum Mode { FORWARD, DGATE, DX, DW };
+enum Mode { FORWARD, SAVE, DGATE, DX, DW };
 
 // A pair of CTAs shares a 256 x 256 tile: each holds its 128 rows of A, half
 // of B's rows and its 128 rows of the accumulator, so a stage costs 32 KB a CTA
@@ -54,8 +60,22 @@ struct Args {
   const void* dh; int64_t dhs;        // DGATE: [M, F], row stride
   void* o0; void* o1;                 // h | dg, du | dx | dWg, dWu
   int M, D, F, act;
+  void* kept; float* kept_scale;      // SAVE: a and b, planes [2][M][F], and their scales
   int tiles_m, tiles_n, half0, ntiles;
 };
+
+// The type a and b are kept in, and whether each row's 64 columns have a scale.
+template <typename T> struct Kept { using type = __half; static constexpr bool scaled = true; };
+template <> struct Kept<__half> { using type = float; static constexpr bool scaled = false; };
+
+// 2^k that brings the largest magnitude into [2^13, 2^14) of f16; 1 where
+// there is none, or an infinity.
+__device__ __forceinline__ float kept_scale_of(float amax) {
+  const int e = (int)(__float_as_uint(amax) >> 23);            // biased exponent, amax >= 0
+  if (amax == 0.0f || e == 255) return 1.0f;
+  const int k = 13 + 127 - e;                                  // -114 .. 140
+  return __uint_as_float((uint32_t)(min(max(k, -126), 126) + 127) << 23);
+}
 
 // ------------------------------------------------------------- activations
 struct ActValue { float act, slope; };
@@ -136,7 +156,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
              const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1,
              const Args a) {
-  constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
+  constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW, PROJ = !B_MN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);   // the leader's count
@@ -193,7 +213,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
           // for the leader's arrival
           const uint32_t bar = cluster_addr(&full[s], 0);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
-          if constexpr (MODE == FORWARD || MODE == DGATE) {
+          if constexpr (PROJ) {
             // the pair's 256 rows of B: the leader's are the gate's, the other's the up's
             tma_load_2d_pair(sa, &tA0, bar, kb * BK, m0);
             tma_load_2d_pair(sb, rank ? &tB1 : &tB0, bar, kb * BK, t.n0);
@@ -253,7 +273,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
       uint32_t v[128];
       const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + b * BN;
       const int row = t.m0 + 32 * q + lane;
-      if constexpr (MODE == FORWARD || MODE == DGATE) {
+      if constexpr (PROJ) {
         // v[0..63] gate and v[64..127] up of columns n0 + 64 side ..
         tmem_ld32(base + 64 * side, v);
         tmem_ld32(base + 64 * side + 32, v + 32);
@@ -267,9 +287,10 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[b], 0));
-      if constexpr (MODE == FORWARD || MODE == DGATE) {
+      if constexpr (PROJ) {
         if (row >= a.M) continue;
         const int n0 = t.n0 + 64 * side;
+        float amax_a = 0.0f, amax_b = 0.0f;
 #pragma unroll
         for (int c = 0; c < 64; c += 8) {
           if (n0 + c >= a.F) break;
@@ -295,6 +316,19 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
 #pragma unroll
             for (int j = 0; j < 8; ++j) o0.set(j, activation<false>(g[j], a.act).act * u[j]);
             o0.store(static_cast<T*>(a.o0) + at);
+          } else if constexpr (MODE == SAVE) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const ActValue f = activation<true>(g[j], a.act);
+              o0.set(j, f.act * u[j]);
+              v[c + j] = __float_as_uint(u[j] * f.slope);
+              v[64 + c + j] = __float_as_uint(f.act);
+              if (Kept<T>::scaled) {
+                amax_a = fmaxf(amax_a, fabsf(u[j] * f.slope));
+                amax_b = fmaxf(amax_b, fabsf(f.act));
+              }
+            }
+            o0.store(static_cast<T*>(a.o0) + at);
           } else {
             load8(static_cast<const T*>(a.dh) + (size_t)row * a.dhs + n0 + c, p);
 #pragma unroll
@@ -305,6 +339,31 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
             }
             o0.store(static_cast<T*>(a.o0) + at);
             o1.store(static_cast<T*>(a.o1) + at);
+          }
+        }
+        if constexpr (MODE == SAVE) {
+          using K = typename Kept<T>::type;
+          const float sa = Kept<T>::scaled ? kept_scale_of(amax_a) : 1.0f;
+          const float sb = Kept<T>::scaled ? kept_scale_of(amax_b) : 1.0f;
+          if (Kept<T>::scaled && n0 < a.F) {
+            const int groups = (a.F + 63) / 64;
+            a.kept_scale[(size_t)row * groups + n0 / 64] = sa;
+            a.kept_scale[(size_t)(a.M + row) * groups + n0 / 64] = sb;
+          }
+          K* ka = static_cast<K*>(a.kept) + (size_t)row * a.F + n0;
+          K* kb = ka + (size_t)a.M * a.F;
+          constexpr int N = 16 / (int)sizeof(K);
+#pragma unroll
+          for (int c = 0; c < 64; c += N) {
+            if (n0 + c >= a.F) break;
+            Pack<K, N> oa, ob;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              oa.set(j, __uint_as_float(v[c + j]) * sa);
+              ob.set(j, __uint_as_float(v[64 + c + j]) * sb);
+            }
+            oa.store(ka + c);
+            ob.store(kb + c);
           }
         }
       } else {
@@ -329,36 +388,80 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
   if (warp == 1) tmem_dealloc_pair(tmem, TMEM_COLS);
 }
 
-// ------------------------------------------------------------- bias gradients
-// Column sums of dg (blockIdx.z 0) and du (1): 256 columns a CTA (eight a
-// lane), its warps taking rows of one chunk in turn; partials [2][chunks][F],
-// joined in a fixed order by column_join_kernel.
-template <typename T>
+// ------------------------------------------------- dg, du and bias gradients
+// From kept a and b (KEPT): dg = dh a, du = dh b, 256 columns a CTA (eight a
+// lane), its warps taking rows of one chunk in turn; with `partial`, the
+// column sums of what was written, joined in a fixed order by
+// column_join_kernel: partials [2][chunks][F]. Without KEPT (dg and du come
+// from the DGATE tiles) the sums alone.
+template <typename T, bool KEPT>
 __global__ void __launch_bounds__(256)
-column_sums_kernel(const T* __restrict__ dg, const T* __restrict__ du, int M, int F,
-                   int chunk_rows, float* __restrict__ partial) {
+gradients_kernel(const T* __restrict__ dh, int64_t dhs, const void* __restrict__ kept,
+                 const float* __restrict__ scale, T* __restrict__ dg, T* __restrict__ du, int M,
+                 int F, int chunk_rows, float* __restrict__ partial) {
+  using K = typename Kept<T>::type;
   __shared__ float acc[8][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c0 = blockIdx.x * 256 + lane * 8;
-  const T* src = blockIdx.z ? du : dg;
   const int r0 = blockIdx.y * chunk_rows, r1 = min(M, r0 + chunk_rows);
-  float s[8] = {};
+  const size_t plane = (size_t)M * F;
+  const int groups = (F + 63) / 64;
+  float sg[8] = {}, su[8] = {};
   if (c0 < F)
+#pragma unroll 2
     for (int r = r0 + warp; r < r1; r += 8) {
-      float p[8];
-      load8(src + (size_t)r * F + c0, p);
+      const size_t at = (size_t)r * F + c0;
+      float g[8], u[8];
+      if constexpr (KEPT) {
+        float d[8], ra = 1.0f, rb = 1.0f;
+        load8(dh + (size_t)r * dhs + c0, d);
+        const K* ka = static_cast<const K*>(kept) + at;
+        if constexpr (Kept<T>::scaled) {
+          load8(ka, g);
+          load8(ka + plane, u);
+          // the scales are powers of two: their reciprocals are exact
+          ra = 1.0f / __ldg(scale + (size_t)r * groups + c0 / 64);
+          rb = 1.0f / __ldg(scale + (size_t)(M + r) * groups + c0 / 64);
+        } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] += p[j];
+          for (int j = 0; j < 8; j += 4) {
+            *reinterpret_cast<float4*>(g + j) = *reinterpret_cast<const float4*>(ka + j);
+            *reinterpret_cast<float4*>(u + j) = *reinterpret_cast<const float4*>(ka + plane + j);
+          }
+        }
+        Pack<T, 8> og, ou;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          og.set(j, d[j] * (g[j] * ra));
+          ou.set(j, d[j] * (u[j] * rb));
+          g[j] = og.get(j);
+          u[j] = ou.get(j);
+        }
+        og.store(dg + at);
+        ou.store(du + at);
+      } else {
+        load8(dg + at, g);
+        load8(du + at, u);
+      }
+      if (partial) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { sg[j] += g[j]; su[j] += u[j]; }
+      }
     }
+  if (!partial) return;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[warp][lane * 8 + j] = s[j];
-  __syncthreads();
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c < F) {
-    float t = 0.0f;
+  for (int z = 0; z < 2; ++z) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) t += acc[w][threadIdx.x];
-    partial[((size_t)blockIdx.z * gridDim.y + blockIdx.y) * F + c] = t;
+    for (int j = 0; j < 8; ++j) acc[warp][lane * 8 + j] = z ? su[j] : sg[j];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < F) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t += acc[w][threadIdx.x];
+      partial[((size_t)z * gridDim.y + blockIdx.y) * F + c] = t;
+    }
+    __syncthreads();
   }
 }
 
@@ -420,8 +523,19 @@ inline int bind_context() {
 
 inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 
+// Kept planes: a and b [2][M][F], 16-byte aligned end to end (F % 8 == 0),
+// then (scaled) the scales f32 [2][M][F / 64 rounded up].
+template <typename T> int64_t kept_bytes(int64_t M, int64_t F) {
+  return 2 * M * F * (int64_t)sizeof(typename Kept<T>::type) +
+         (Kept<T>::scaled ? 2 * M * ((F + 63) / 64) * 4 : 0);
+}
+template <typename T> float* kept_scales(void* kept, int64_t M, int64_t F) {
+  return reinterpret_cast<float*>(static_cast<uint8_t*>(kept) +
+                                  2 * M * F * sizeof(typename Kept<T>::type));
+}
+
 template <typename T>
-int projections(bool dgate, const void* x, int64_t xs, const void* wg, const void* wu, Args a,
+int projections(Mode mode, const void* x, int64_t xs, const void* wg, const void* wu, Args a,
                 cudaStream_t st) {
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   if (int rc = bind_context()) return rc;
@@ -432,13 +546,15 @@ int projections(bool dgate, const void* x, int64_t xs, const void* wg, const voi
   a.tiles_m = cdiv(a.M, 2 * BM);
   a.tiles_n = cdiv(a.F, BN / 2);
   a.ntiles = a.tiles_m * a.tiles_n;
-  return dgate ? launch<DGATE, T>(tx, tx, tg, tu, a, st) : launch<FORWARD, T>(tx, tx, tg, tu, a, st);
+  if (mode == DGATE) return launch<DGATE, T>(tx, tx, tg, tu, a, st);
+  if (mode == SAVE) return launch<SAVE, T>(tx, tx, tg, tu, a, st);
+  return launch<FORWARD, T>(tx, tx, tg, tu, a, st);
 }
 
-// Chunks of rows of the bias gradient's column sums: about four CTAs a
-// multiprocessor, at least 32 rows each.
+// Chunks of rows of gradients_kernel: about eight CTAs a multiprocessor, at
+// least 32 rows each.
 inline int bias_chunks(int M, int F) {
-  const int tiles = cdiv(F, 256) * 2, want = cdiv(148 * 4, tiles), most = cdiv(M, 32);
+  const int tiles = cdiv(F, 256), want = cdiv(148 * 8, tiles), most = cdiv(M, 32);
   return want < most ? (want > 0 ? want : 1) : (most > 0 ? most : 1);
 }
 
@@ -454,7 +570,18 @@ int backward(const GatedBackward& w, cudaStream_t st) {
   Args a{};
   a.bg = w.bg; a.bu = w.bu; a.dh = w.dh; a.dhs = w.dhs; a.o0 = dg; a.o1 = du;
   a.M = M; a.D = D; a.F = F; a.act = w.act;
-  if (int rc = projections<T>(true, w.x, w.xs, w.wg, w.wu, a, st)) return rc;
+  const int chunks = bias_chunks(M, F);
+  const bool bias = w.dbg || w.dbu;
+  const dim3 grid(cdiv(F, 256), chunks);
+  if (int rc = bind_context()) return rc;
+  if (w.kept) {
+    gradients_kernel<T, true><<<grid, 256, 0, st>>>(
+        static_cast<const T*>(w.dh), w.dhs, w.kept, kept_scales<T>(w.kept, M, F),
+        static_cast<T*>(dg), static_cast<T*>(du), M, F, cdiv(M, chunks), bias ? partial : nullptr);
+    if (int rc = launch_status()) return rc;
+  } else {
+    if (int rc = projections<T>(DGATE, w.x, w.xs, w.wg, w.wu, a, st)) return rc;
+  }
   if (w.dx) {
     CUtensorMap ag, au, bgm, bum;
     if (int rc = tmap16(&ag, dg, bf, F, M, F, BM)) return rc;
@@ -482,11 +609,13 @@ int backward(const GatedBackward& w, cudaStream_t st) {
     c.ntiles = c.tiles_m * c.tiles_n;
     if (int rc = launch<DW, T>(ag, au, bx, bx, c, st)) return rc;
   }
-  if (w.dbg || w.dbu) {
-    const int chunks = bias_chunks(M, F);
-    column_sums_kernel<T><<<dim3(cdiv(F, 256), chunks, 2), 256, 0, st>>>(
-        static_cast<const T*>(dg), static_cast<const T*>(du), M, F, cdiv(M, chunks), partial);
-    if (int rc = launch_status()) return rc;
+  if (bias) {
+    if (!w.kept) {
+      gradients_kernel<T, false><<<grid, 256, 0, st>>>(nullptr, 0, nullptr, nullptr,
+                                                       static_cast<T*>(dg), static_cast<T*>(du), M,
+                                                       F, cdiv(M, chunks), partial);
+      if (int rc = launch_status()) return rc;
+    }
     column_join_kernel<T><<<dim3(cdiv(F, 256), 2), 256, 0, st>>>(
         partial, chunks, F, static_cast<T*>(w.dbg), static_cast<T*>(w.dbu));
     return launch_status();
@@ -501,13 +630,25 @@ int64_t gated_backward_work(int M, int F) {
   return 2 * plane + (int64_t)2 * gated::bias_chunks(M, F) * F * 4;
 }
 
+int64_t gated_kept_bytes(int64_t M, int64_t F, int dtype) {
+  return dtype == GWB_BF16 ? gated::kept_bytes<__nv_bfloat16>(M, F) : gated::kept_bytes<__half>(M, F);
+}
+
+template <typename T>
+static int gated_forward(const void* x, int64_t xs, const void* wg, const void* wu, gated::Args a,
+                         void* kept, cudaStream_t st) {
+  a.kept = kept;
+  if (kept) a.kept_scale = gated::kept_scales<T>(kept, a.M, a.F);
+  return gated::projections<T>(kept ? gated::SAVE : gated::FORWARD, x, xs, wg, wu, a, st);
+}
+
 int launch_gated_forward(const void* x, int64_t xs, const void* wg, const void* wu, const void* bg,
                          const void* bu, int M, int D, int F, int act, int dtype, void* h,
-                         cudaStream_t st) {
+                         void* kept, cudaStream_t st) {
   gated::Args a{};
   a.bg = bg; a.bu = bu; a.o0 = h; a.M = M; a.D = D; a.F = F; a.act = act;
-  return dtype == GWB_BF16 ? gated::projections<__nv_bfloat16>(false, x, xs, wg, wu, a, st)
-                           : gated::projections<__half>(false, x, xs, wg, wu, a, st);
+  return dtype == GWB_BF16 ? gated_forward<__nv_bfloat16>(x, xs, wg, wu, a, kept, st)
+                           : gated_forward<__half>(x, xs, wg, wu, a, kept, st);
 }
 
 int launch_gated_backward(const GatedBackward& w, int dtype, cudaStream_t st) {

@@ -26,6 +26,7 @@ struct GatedBackward {
   const void* wg; const void* wu; const void* bg; const void* bu;
   int M, D, F, act;
   void* dx; void* dwg; void* dwu; void* dbg; void* dbu;   // any may be null
+  void* kept;                      // from the forward call, or null: computed again
   void* work;
 };
 int launch_act_int4(const void* x, const void* smooth, const void* down_t, void* codes,

@@ -550,8 +550,8 @@ GatedShape gated_shape(const Tensor& x, const Tensor& wg, const Tensor& wu, cons
   return g;
 }
 
-Tensor gated_linear_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu, const OptTensor& bg,
-                         const OptTensor& bu, int64_t act) {
+Tensor gated_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const OptTensor& bg,
+                     const OptTensor& bu, int64_t act, Tensor* kept) {
   const GatedShape g = gated_shape(x, wg, wu, bg, bu, act);
   const c10::cuda::CUDAGuard guard(x.device());
   int64_t xs = 0;
@@ -559,17 +559,39 @@ Tensor gated_linear_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu, co
   auto shape = x.sizes().vec();
   shape.back() = g.f;
   Tensor h = at::empty(shape, x.options().memory_format(at::MemoryFormat::Contiguous));
-  check_status(gwb_gated_linear(xr.const_data_ptr(), xs, wg.const_data_ptr(), wu.const_data_ptr(),
-                                ptr(bg), ptr(bu), g.rows, g.d, g.f, (int)act, g.dtype,
-                                h.data_ptr(), stream_of(x)),
-               "gated_linear");
+  if (!kept) {
+    check_status(gwb_gated_linear(xr.const_data_ptr(), xs, wg.const_data_ptr(),
+                                  wu.const_data_ptr(), ptr(bg), ptr(bu), g.rows, g.d, g.f,
+                                  (int)act, g.dtype, h.data_ptr(), stream_of(x)),
+                 "gated_linear");
+    return h;
+  }
+  *kept = at::empty({gwb_gated_linear_kept(g.rows, g.f, g.dtype)}, x.options().dtype(at::kByte));
+  check_status(gwb_gated_linear_keep(xr.const_data_ptr(), xs, wg.const_data_ptr(),
+                                     wu.const_data_ptr(), ptr(bg), ptr(bu), g.rows, g.d, g.f,
+                                     (int)act, g.dtype, h.data_ptr(), kept->data_ptr(),
+                                     stream_of(x)),
+               "gated_linear_keep");
   return h;
+}
+
+Tensor gated_linear_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu, const OptTensor& bg,
+                         const OptTensor& bu, int64_t act, bool recompute) {
+  return gated_forward(x, wg, wu, bg, bu, act, nullptr);
+}
+
+std::tuple<Tensor, Tensor> gated_linear_keep_cuda(const Tensor& x, const Tensor& wg,
+                                                  const Tensor& wu, const OptTensor& bg,
+                                                  const OptTensor& bu, int64_t act) {
+  Tensor kept;
+  Tensor h = gated_forward(x, wg, wu, bg, bu, act, &kept);
+  return {h, kept};
 }
 
 // -> (dx, dw_gate, dw_up, db_gate, db_up); one not asked for is empty [0]
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward_cuda(
     const Tensor& dh, const Tensor& x, const Tensor& wg, const Tensor& wu, const OptTensor& bg,
-    const OptTensor& bu, int64_t act, std::array<bool, 5> mask) {
+    const OptTensor& bu, const OptTensor& kept, int64_t act, std::array<bool, 5> mask) {
   const GatedShape g = gated_shape(x, wg, wu, bg, bu, act);
   const c10::cuda::CUDAGuard guard(x.device());
   need_on(dh, "dh", x);
@@ -578,6 +600,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward_cuda(
        "dh must be ", x.scalar_type(), " of x's shape with ", g.f, " features, got ", dh.sizes());
   NEED((!mask[3] || has(bg)) && (!mask[4] || has(bu)),
        "a gradient was asked for of a bias that is not given");
+  if (has(kept)) {
+    need_on(*kept, "kept", x);
+    NEED(kept->scalar_type() == at::kByte && kept->dim() == 1 && kept->is_contiguous() &&
+             aligned16(*kept) && kept->size(0) == gwb_gated_linear_kept(g.rows, g.f, g.dtype),
+         "kept must be what gated_linear_keep gave for x and the weights");
+  }
   int64_t xs = 0, ds = 0;
   const Tensor xr = tma_rows_of(x, &xs), dr = tma_rows_of(dh, &ds);
   const auto out = [&](bool on, at::IntArrayRef shape) {
@@ -591,8 +619,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward_cuda(
   const auto at_ = [](bool on, Tensor& t) { return on ? t.data_ptr() : nullptr; };
   check_status(gwb_gated_linear_backward(
                    dr.const_data_ptr(), ds, xr.const_data_ptr(), xs, wg.const_data_ptr(),
-                   wu.const_data_ptr(), ptr(bg), ptr(bu), g.rows, g.d, g.f, (int)act, g.dtype,
-                   at_(mask[0], dx), at_(mask[1], dwg), at_(mask[2], dwu), at_(mask[3], dbg),
+                   wu.const_data_ptr(), ptr(bg), ptr(bu), has(kept) ? kept->data_ptr() : nullptr, g.rows,
+                   g.d, g.f, (int)act, g.dtype, at_(mask[0], dx), at_(mask[1], dwg), at_(mask[2], dwu), at_(mask[3], dbg),
                    at_(mask[4], dbu), work.data_ptr(), stream_of(x)),
                "gated_linear_backward");
   return {dx, dwg, dwu, dbg, dbu};
@@ -600,38 +628,47 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward_cuda(
 
 struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu,
-                        const OptTensor& bg, const OptTensor& bu, int64_t act) {
+                        const OptTensor& bg, const OptTensor& bu, int64_t act, bool recompute) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = op_of<decltype(gated_linear_cuda)>("gwb200::gated_linear");
-    Tensor h = op.call(x, wg, wu, bg, bu, act);
-    ctx->save_for_backward({x, wg, wu, has(bg) ? *bg : Tensor(), has(bu) ? *bu : Tensor()});
+    Tensor h, kept;
+    if (recompute) {
+      static auto op = op_of<decltype(gated_linear_cuda)>("gwb200::gated_linear");
+      h = op.call(x, wg, wu, bg, bu, act, true);
+    } else {
+      static auto op = op_of<decltype(gated_linear_keep_cuda)>("gwb200::gated_linear_keep");
+      std::tie(h, kept) = op.call(x, wg, wu, bg, bu, act);
+    }
+    ctx->save_for_backward(
+        {x, wg, wu, has(bg) ? *bg : Tensor(), has(bu) ? *bu : Tensor(), kept});
     ctx->saved_data["act"] = act;
     return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto v = ctx->get_saved_variables();
     refuse_second_order("gated_linear_backward", grads[0], v[0], v[1], v[2], v[3], v[4]);
-    if (!grads[0].defined()) return variable_list(6);
+    if (!grads[0].defined()) return variable_list(7);
     std::array<bool, 5> mask{};
     for (int i = 0, given = 0; i < 5; ++i)
       if (v[i].defined()) mask[i] = ctx->needs_input_grad(given++);
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = op_of<decltype(gated_linear_backward_cuda)>("gwb200::gated_linear_backward");
-    auto [dx, dwg, dwu, dbg, dbu] = op.call(grads[0], v[0], v[1], v[2], opt(v[3]), opt(v[4]),
-                                            ctx->saved_data["act"].toInt(), mask);
+    auto [dx, dwg, dwu, dbg, dbu] =
+        op.call(grads[0], v[0], v[1], v[2], opt(v[3]), opt(v[4]), opt(v[5]),
+                ctx->saved_data["act"].toInt(), mask);
     const auto give = [&](int i, Tensor& t) { return mask[i] ? t : Tensor(); };
-    return {give(0, dx), give(1, dwg), give(2, dwu), give(3, dbg), give(4, dbu), Tensor()};
+    return {give(0, dx), give(1, dwg), give(2, dwu), give(3, dbg), give(4, dbu), Tensor(), Tensor()};
   }
 };
 
 Tensor gated_linear_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu,
-                             const OptTensor& bg, const OptTensor& bu, int64_t act) {
+                             const OptTensor& bg, const OptTensor& bu, int64_t act,
+                             bool recompute) {
   if (at::GradMode::is_enabled() &&
       (wants(x) || wants(wg) || wants(wu) || wants(bg) || wants(bu)))
-    return GatedLinearFn::apply(x, wg, wu, bg, bu, act);
+    return GatedLinearFn::apply(x, wg, wu, bg, bu, act, recompute);
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = op_of<decltype(gated_linear_cuda)>("gwb200::gated_linear");
-  return op.call(x, wg, wu, bg, bu, act);
+  return op.call(x, wg, wu, bg, bu, act, recompute);
 }
 
 }  // namespace gwb200_block
@@ -649,9 +686,11 @@ TORCH_LIBRARY_FRAGMENT(gwb200, m) {
   m.def("rotary_(Tensor(a!) q, Tensor(b!)? k, Tensor positions, Tensor inv_freq, Tensor? axis, "
         "bool interleaved, float scale, bool inverse) -> ()");
   m.def("gated_linear(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, "
-        "int activation) -> Tensor");
+        "int activation, bool recompute) -> Tensor");
+  m.def("gated_linear_keep(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, "
+        "int activation) -> (Tensor, Tensor)");
   m.def("gated_linear_backward(Tensor dh, Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, "
-        "Tensor? b_up, int activation, bool[5] mask) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+        "Tensor? b_up, Tensor? kept, int activation, bool[5] mask) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(gwb200, CUDA, m) {
@@ -661,6 +700,7 @@ TORCH_LIBRARY_IMPL(gwb200, CUDA, m) {
   m.impl("rotary", &gwb200_block::rotary_cuda);
   m.impl("rotary_", &gwb200_block::rotary_inplace_cuda);
   m.impl("gated_linear", &gwb200_block::gated_linear_cuda);
+  m.impl("gated_linear_keep", &gwb200_block::gated_linear_keep_cuda);
   m.impl("gated_linear_backward", &gwb200_block::gated_linear_backward_cuda);
 }
 

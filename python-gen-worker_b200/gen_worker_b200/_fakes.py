@@ -36,11 +36,19 @@ def _(q, k, positions, inv_freq, axis, interleaved, scale, inverse):
 
 
 @torch.library.register_fake("gwb200::gated_linear")
-def _(x, w_gate, w_up, b_gate, b_up, activation):
+def _(x, w_gate, w_up, b_gate, b_up, activation, recompute):
     return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
 
 
+@torch.library.register_fake("gwb200::gated_linear_keep")
+def _(x, w_gate, w_up, b_gate, b_up, activation):
+    f = w_gate.shape[0]
+    rows = x.numel() // x.shape[-1]
+    kept = rows * f * 4 + rows * ((f + 63) // 64) * 8 if x.dtype == torch.bfloat16 else rows * f * 8
+    return x.new_empty((*x.shape[:-1], f)), x.new_empty(kept, dtype=torch.uint8)
+
+
 @torch.library.register_fake("gwb200::gated_linear_backward")
-def _(dh, x, w_gate, w_up, b_gate, b_up, activation, mask):
+def _(dh, x, w_gate, w_up, b_gate, b_up, kept, activation, mask):
     given = (x, w_gate, w_up, b_gate, b_up)
     return tuple(t.new_empty(t.shape) if on else x.new_empty(0) for t, on in zip(given, mask))

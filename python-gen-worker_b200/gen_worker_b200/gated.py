@@ -24,21 +24,23 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                  b_gate: Optional[torch.Tensor] = None, b_up: Optional[torch.Tensor] = None, *,
-                 activation: str = "silu") -> torch.Tensor:
+                 activation: str = "silu", recompute: bool = False) -> torch.Tensor:
     """x [..., D], w_gate / w_up [F, D], biases [F] or None, all bfloat16 or
     all float16 -> h [..., F], contiguous. D and F are multiples of 8; weights
     and biases contiguous and 16-byte aligned (halves of a fused weight are).
     x may be a slice of wider rows; rows that 16-byte loads cannot step
     through are copied first. f32 accumulation, one rounding. Differentiable
-    once in all of them; the backward pass computes the projections again
-    instead of keeping them."""
+    once in all of them. Where a gradient is wanted, 4 bytes per element of h
+    (bfloat16; 8 for float16) are kept for the backward pass, or, with
+    ``recompute``, nothing, and it computes the projections again."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise SvdqB200Error(f"activation {activation!r} is not one of {sorted(ACTIVATIONS)}")
     if not x.is_cuda:
         raise SvdqB200Error(f"x must be a CUDA tensor (no CPU path), got {x.device}")
     try:
-        return native.block_ops(x).gated_linear(x, w_gate, w_up, b_gate, b_up, code)
+        return native.block_ops(x).gated_linear(x, w_gate, w_up, b_gate, b_up, code,
+                                                recompute)
     except ValueError as exc:
         raise SvdqB200Error(f"gated_linear: {exc}") from None
 
@@ -46,11 +48,12 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
 class GatedFeedForward(nn.Module):
     """``down(gated_linear(x))`` with parameters ``w_gate`` / ``w_up``
     [hidden, dim] and, with ``bias``, ``b_gate`` / ``b_up`` [hidden]; ``down``
-    is any module from hidden features (None: h itself is returned)."""
+    is any module from hidden features (None: h itself is returned);
+    ``recompute`` as in :func:`gated_linear`."""
 
     def __init__(self, dim: int, hidden: int, *, activation: str = "silu", bias: bool = False,
-                 down: Optional[nn.Module] = None, dtype: Any = torch.bfloat16,
-                 device: Any = None) -> None:
+                 down: Optional[nn.Module] = None, recompute: bool = False,
+                 dtype: Any = torch.bfloat16, device: Any = None) -> None:
         super().__init__()
         if activation not in ACTIVATIONS:
             raise SvdqB200Error(f"activation {activation!r} is not one of {sorted(ACTIVATIONS)}")
@@ -70,10 +73,11 @@ class GatedFeedForward(nn.Module):
         self.b_gate = param(hidden) if bias else None
         self.b_up = param(hidden) if bias else None
         self.down = down
+        self.recompute = bool(recompute)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         h = gated_linear(x, self.w_gate, self.w_up, self.b_gate, self.b_up,
-                         activation=self.activation)
+                         activation=self.activation, recompute=self.recompute)
         return h if self.down is None else self.down(h)
 
     def extra_repr(self) -> str:

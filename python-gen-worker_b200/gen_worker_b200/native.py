@@ -87,9 +87,12 @@ _SIGNATURES = {
                    c_i64, c_i64, ctypes.c_float, c_int, c_int, c_int, c_void_p],
     "gwb_gated_linear": [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64,
                          c_i64, c_int, c_int, c_void_p, c_void_p],
+    "gwb_gated_linear_keep": [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64,
+                              c_i64, c_int, c_int, c_void_p, c_void_p, c_void_p],
+    "gwb_gated_linear_kept": [c_i64, c_i64, c_int],
     "gwb_gated_linear_backward_work": [c_i64, c_i64],
     "gwb_gated_linear_backward": [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
-                                  c_void_p, c_i64, c_i64, c_i64, c_int, c_int, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_i64, c_i64, c_i64, c_int, c_int, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "gwb_fp8_gemm": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64,
                      c_int, c_void_p, c_void_p],
@@ -106,7 +109,8 @@ _SIGNATURES = {
     "gwb_status_string": [c_int],
 }
 
-_RETURNS_I64 = {"gwb_layer_norm_backward_work", "gwb_gated_linear_backward_work"}
+_RETURNS_I64 = {"gwb_layer_norm_backward_work", "gwb_gated_linear_backward_work",
+                "gwb_gated_linear_kept"}
 EXPORTED = tuple(_SIGNATURES)
 
 

@@ -42,8 +42,14 @@ def verify(p, act, h, grads):
     want = dict(zip(names, torch.autograd.grad(h64, [r[n] for n in names], p["dh"].double())))
     x, wg, wu = (p[n].double().abs() for n in ("x", "w_gate", "w_up"))
     tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
-    eg = m["dg"] + half_step(dtype) * (dg.abs() + m["dg"]) + tiny
-    eu = m["du"] + half_step(dtype) * (du.abs() + m["du"]) + tiny
+    # bf16: a and b are kept as f16 times a power of two per 64 columns, off by
+    # half a step of f16 or, far below the largest of the 64, 2^-39 of that
+    kept = half_step(torch.float16) if dtype == torch.bfloat16 else 0.0
+    dh = p["dh"].double().abs()
+    low = 2.0 ** -38 if dtype == torch.bfloat16 else 0.0
+    far_a, far_b = (dh * (t.abs() / dh.clamp(min=1e-30)).amax(1, keepdim=True) for t in (dg, du))
+    eg = m["dg"] + (half_step(dtype) + kept) * (dg.abs() + m["dg"]) + low * far_a + tiny
+    eu = m["du"] + (half_step(dtype) + kept) * (du.abs() + m["du"]) + low * far_b + tiny
     rows, f = dg.shape
     err = {"x": eg @ wg + eu @ wu + (2 * f + 2) * U * ((dg.abs() + eg) @ wg + (du.abs() + eu) @ wu),
            "w_gate": eg.t() @ x + (rows + 2) * U * ((dg.abs() + eg).t() @ x),
@@ -55,7 +61,7 @@ def verify(p, act, h, grads):
         assert got.dtype == dtype
 
 
-def run(p, act="silu", names=None):
+def run(p, act="silu", names=None, recompute=False):
     from gen_worker_b200 import gated_linear
 
     names = names or [n for n in ("x", "w_gate", "w_up", "b_gate", "b_up") if n in p]
@@ -63,7 +69,7 @@ def run(p, act="silu", names=None):
     for n in names:
         dev[n].requires_grad_(True)
     h = gated_linear(dev["x"], dev["w_gate"], dev["w_up"], dev.get("b_gate"), dev.get("b_up"),
-                     activation=act)
+                     activation=act, recompute=recompute)
     return h, dict(zip(names, torch.autograd.grad(h, [dev[n] for n in names], dev["dh"])))
 
 
@@ -84,17 +90,20 @@ def test_sizes(cuda_ready, m, d, f, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("m", [3, 150])
-def test_activations_and_biases(cuda_ready, m, act, dtype):
+@pytest.mark.parametrize("recompute", [False, True])
+def test_activations_and_biases(cuda_ready, recompute, m, act, dtype):
     p = make(m, 320, 264, dtype, bias=True)
     p["x"][0] *= 12                                # far into both tails
-    verify(p, act, *run(p, act))
+    p["x"][1] *= 2.0 ** -9                         # far below the kept planes' usual scale
+    verify(p, act, *run(p, act, recompute=recompute))
 
 
 @pytest.mark.gpu
 def test_many_tiles(cuda_ready):
     """More tiles than multiprocessors, so the persistent walk wraps."""
     p = make(1100, 520, 2600, torch.bfloat16, bias=True)
-    verify(p, "gelu_tanh", *run(p, "gelu_tanh"))
+    for recompute in (False, True):
+        verify(p, "gelu_tanh", *run(p, "gelu_tanh", recompute=recompute))
 
 
 @pytest.mark.gpu
