@@ -82,25 +82,27 @@ struct ActValue { float act, slope; };
 
 // act(g), and act'(g) when SLOPE. silu and the tanh form of GELU are
 // g * sigmoid(t): 1 - sigmoid is taken without cancellation on either side.
-template <bool SLOPE>
-__device__ __forceinline__ ActValue activation(float g, int kind) {
+// KIND is a template argument: a branch an element would keep the compiler
+// from running the elements' exp and divide chains side by side.
+template <int KIND, bool SLOPE>
+__device__ __forceinline__ ActValue activation(float g) {
   ActValue r;
   r.slope = 0.0f;
-  if (kind == GWB_ACT_GELU) {
+  if constexpr (KIND == GWB_ACT_GELU) {
     const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
     r.act = g * cdf;
     if (SLOPE) r.slope = cdf + g * (0.39894228040143268f * __expf(-0.5f * g * g));
-    return r;
-  }
-  constexpr float c = 2.0f * 0.79788456080286536f, k = 0.044715f;   // 2 sqrt(2 / pi)
-  const float t = kind == GWB_ACT_SILU ? g : c * (g + k * g * g * g);
-  const float e = __expf(-t);
-  const float s = __fdividef(1.0f, 1.0f + e);
-  r.act = g * s;
-  if (SLOPE) {
-    const float q = t >= 0.0f ? e * s : 1.0f - s;                   // 1 - s
-    const float dt = kind == GWB_ACT_SILU ? 1.0f : c * (1.0f + 3.0f * k * g * g);
-    r.slope = s + g * (s * q) * dt;
+  } else {
+    constexpr float c = 2.0f * 0.79788456080286536f, k = 0.044715f;   // 2 sqrt(2 / pi)
+    const float t = KIND == GWB_ACT_SILU ? g : c * (g + k * g * g * g);
+    const float e = __expf(-t);
+    const float s = __fdividef(1.0f, 1.0f + e);
+    r.act = g * s;
+    if (SLOPE) {
+      const float q = t >= 0.0f ? e * s : 1.0f - s;                   // 1 - s
+      const float dt = KIND == GWB_ACT_SILU ? 1.0f : c * (1.0f + 3.0f * k * g * g);
+      r.slope = s + g * (s * q) * dt;
+    }
   }
   return r;
 }
@@ -143,15 +145,29 @@ __device__ __forceinline__ void land_copies() {
   while (clock64() - t < 2000000) { }
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void load8(const T* p, float (&f)[N]) {
-  Pack<T, 8> v;
-  v.load(p);
+// Eight 16-bit elements <-> f32, two at a time
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  F2 v[4];
+  unpack<T>(*reinterpret_cast<const uint4*>(p), v);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = v.get(j);
+  for (int j = 0; j < 4; ++j) {
+    const float2 s = split(v[j]);
+    f[2 * j] = s.x;
+    f[2 * j + 1] = s.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 round8(const float (&f)[8]) {
+  const F2 v[4] = {f2(f[0], f[1]), f2(f[2], f[3]), f2(f[4], f[5]), f2(f[6], f[7])};
+  return repack<T>(v);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(p) = round8<T>(f);
 }
 
-template <int MODE, typename T>
+template <int MODE, int ACT, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
              const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1,
@@ -311,35 +327,34 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
             for (int j = 0; j < 8; ++j) u[j] += p[j];
           }
           const size_t at = (size_t)row * a.F + n0 + c;
-          Pack<T, 8> o0, o1;
+          float o0[8], o1[8];
           if constexpr (MODE == FORWARD) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o0.set(j, activation<false>(g[j], a.act).act * u[j]);
-            o0.store(static_cast<T*>(a.o0) + at);
+            for (int j = 0; j < 8; ++j) o0[j] = activation<ACT, false>(g[j]).act * u[j];
           } else if constexpr (MODE == SAVE) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const ActValue f = activation<true>(g[j], a.act);
-              o0.set(j, f.act * u[j]);
-              v[c + j] = __float_as_uint(u[j] * f.slope);
+              const ActValue f = activation<ACT, true>(g[j]);
+              o0[j] = f.act * u[j];
+              const float fa = u[j] * f.slope;
+              v[c + j] = __float_as_uint(fa);
               v[64 + c + j] = __float_as_uint(f.act);
               if (Kept<T>::scaled) {
-                amax_a = fmaxf(amax_a, fabsf(u[j] * f.slope));
+                amax_a = fmaxf(amax_a, fabsf(fa));
                 amax_b = fmaxf(amax_b, fabsf(f.act));
               }
             }
-            o0.store(static_cast<T*>(a.o0) + at);
           } else {
             load8(static_cast<const T*>(a.dh) + (size_t)row * a.dhs + n0 + c, p);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const ActValue f = activation<true>(g[j], a.act);
-              o0.set(j, p[j] * u[j] * f.slope);
-              o1.set(j, p[j] * f.act);
+              const ActValue f = activation<ACT, true>(g[j]);
+              o0[j] = p[j] * u[j] * f.slope;
+              o1[j] = p[j] * f.act;
             }
-            o0.store(static_cast<T*>(a.o0) + at);
-            o1.store(static_cast<T*>(a.o1) + at);
+            store8(static_cast<T*>(a.o1) + at, o1);
           }
+          store8(static_cast<T*>(a.o0) + at, o0);
         }
         if constexpr (MODE == SAVE) {
           using K = typename Kept<T>::type;
@@ -352,18 +367,25 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
           }
           K* ka = static_cast<K*>(a.kept) + (size_t)row * a.F + n0;
           K* kb = ka + (size_t)a.M * a.F;
-          constexpr int N = 16 / (int)sizeof(K);
 #pragma unroll
-          for (int c = 0; c < 64; c += N) {
+          for (int c = 0; c < 64; c += 8) {
             if (n0 + c >= a.F) break;
-            Pack<K, N> oa, ob;
+            float oa[8], ob[8];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-              oa.set(j, __uint_as_float(v[c + j]) * sa);
-              ob.set(j, __uint_as_float(v[64 + c + j]) * sb);
+            for (int j = 0; j < 8; ++j) {
+              oa[j] = __uint_as_float(v[c + j]) * sa;
+              ob[j] = __uint_as_float(v[64 + c + j]) * sb;
             }
-            oa.store(ka + c);
-            ob.store(kb + c);
+            if constexpr (sizeof(K) == 2) {
+              store8(ka + c, oa);
+              store8(kb + c, ob);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; j += 4) {
+                *reinterpret_cast<float4*>(ka + c + j) = make_float4(oa[j], oa[j + 1], oa[j + 2], oa[j + 3]);
+                *reinterpret_cast<float4*>(kb + c + j) = make_float4(ob[j], ob[j + 1], ob[j + 2], ob[j + 3]);
+              }
+            }
           }
         }
       } else {
@@ -373,10 +395,10 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
 #pragma unroll
         for (int c = 0; c < 128; c += 8) {
           if (n0 + c >= a.D) break;
-          Pack<T, 8> o;
+          float o[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o.set(j, __uint_as_float(v[c + j]));
-          o.store(out + n0 + c);
+          for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(v[c + j]);
+          store8(out + n0 + c, o);
         }
       }
     }
@@ -429,16 +451,18 @@ gradients_kernel(const T* __restrict__ dh, int64_t dhs, const void* __restrict__
             *reinterpret_cast<float4*>(u + j) = *reinterpret_cast<const float4*>(ka + plane + j);
           }
         }
-        Pack<T, 8> og, ou;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          og.set(j, d[j] * (g[j] * ra));
-          ou.set(j, d[j] * (u[j] * rb));
-          g[j] = og.get(j);
-          u[j] = ou.get(j);
+          g[j] = d[j] * (g[j] * ra);
+          u[j] = d[j] * (u[j] * rb);
         }
-        og.store(dg + at);
-        ou.store(du + at);
+        const uint4 rg = round8<T>(g), ru = round8<T>(u);
+        *reinterpret_cast<uint4*>(dg + at) = rg;
+        *reinterpret_cast<uint4*>(du + at) = ru;
+        if (partial) {
+          load8(reinterpret_cast<const T*>(&rg), g);
+          load8(reinterpret_cast<const T*>(&ru), u);
+        }
       } else {
         load8(dg + at, g);
         load8(du + at, u);
@@ -492,10 +516,10 @@ inline int tmap16(CUtensorMap* m, const void* base, bool bf16, int64_t cols, int
   return r == CUDA_SUCCESS ? GWB_SUCCESS : GWB_E_TMAP;
 }
 
-template <int MODE, typename T>
+template <int MODE, int ACT, typename T>
 int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0,
            const CUtensorMap& b1, Args a, cudaStream_t st) {
-  auto kern = gated_kernel<MODE, T>;
+  auto kern = gated_kernel<MODE, ACT, T>;
   // the shared-memory limit is a property of the function on each device
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
@@ -546,9 +570,15 @@ int projections(Mode mode, const void* x, int64_t xs, const void* wg, const void
   a.tiles_m = cdiv(a.M, 2 * BM);
   a.tiles_n = cdiv(a.F, BN / 2);
   a.ntiles = a.tiles_m * a.tiles_n;
-  if (mode == DGATE) return launch<DGATE, T>(tx, tx, tg, tu, a, st);
-  if (mode == SAVE) return launch<SAVE, T>(tx, tx, tg, tu, a, st);
-  return launch<FORWARD, T>(tx, tx, tg, tu, a, st);
+  const auto go = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    if (mode == DGATE) return launch<DGATE, ACT, T>(tx, tx, tg, tu, a, st);
+    if (mode == SAVE) return launch<SAVE, ACT, T>(tx, tx, tg, tu, a, st);
+    return launch<FORWARD, ACT, T>(tx, tx, tg, tu, a, st);
+  };
+  if (a.act == GWB_ACT_SILU) return go(std::integral_constant<int, GWB_ACT_SILU>{});
+  if (a.act == GWB_ACT_GELU) return go(std::integral_constant<int, GWB_ACT_GELU>{});
+  return go(std::integral_constant<int, GWB_ACT_GELU_TANH>{});
 }
 
 // Chunks of rows of gradients_kernel: about eight CTAs a multiprocessor, at
@@ -593,7 +623,7 @@ int backward(const GatedBackward& w, cudaStream_t st) {
     c.tiles_m = cdiv(M, 2 * BM);
     c.tiles_n = cdiv(D, BN);
     c.ntiles = c.tiles_m * c.tiles_n;
-    if (int rc = launch<DX, T>(ag, au, bgm, bum, c, st)) return rc;
+    if (int rc = launch<DX, 0, T>(ag, au, bgm, bum, c, st)) return rc;
   }
   if (w.dwg || w.dwu) {
     CUtensorMap ag, au, bx;
@@ -607,7 +637,7 @@ int backward(const GatedBackward& w, cudaStream_t st) {
     c.tiles_m = cdiv(F, 2 * BM) * (w.dwg && w.dwu ? 2 : 1);
     c.tiles_n = cdiv(D, BN);
     c.ntiles = c.tiles_m * c.tiles_n;
-    if (int rc = launch<DW, T>(ag, au, bx, bx, c, st)) return rc;
+    if (int rc = launch<DW, 0, T>(ag, au, bx, bx, c, st)) return rc;
   }
   if (bias) {
     if (!w.kept) {
