@@ -413,34 +413,45 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
 
 // ------------------------------------------------------------- few rows
 // Up to 128 rows: reading the weights bounds it. The weights are the MMA's A
-// operand, 64 gate rows and the same 64 up rows to its 128, and x its B operand
-// with the rows rounded up to 16: a tile's features are then TMEM lanes, which
-// all have work however few the rows are, and consecutive lanes store
-// consecutive features. Tiles of 64 features keep every multiprocessor
-// streaming; up to eleven stages of weights are in flight in each.
-// 0 TMA, 1 MMA, 2-3 idle, 4-11 epilogue: lane quarters 0 and 1 hold the gate
-// and finish, 2 and 3 hold the up and pass it through shared memory; each half
-// of the eight takes half of the rows.
+// operand and x its B operand with the rows rounded up to 16: features are then
+// TMEM lanes, which all have work however few the rows are, and consecutive
+// lanes store consecutive features. A tile has `w` features, a multiple of 8
+// that gives the multiprocessors equal numbers of tiles (with 64 always, 192
+// tiles of 12288 features took 39 us on 148 of them, with 88 and 140 tiles 31);
+// lanes beyond w hold what is left in shared memory and store nothing.
+//   FT 128  w over 64: gate and up rows are two A operands with an accumulator
+//           each, side by side;
+//   FT 64   up to 64: they are halves of one A operand, half the MMAs: lane
+//           quarters 0 and 1 hold the gate and finish, 2 and 3 hold the up and
+//           pass it through shared memory.
+// Warps: 0 TMA, 1 MMA, 2-3 idle, 4-11 epilogue; each half of the eight takes 16
+// rows of x in turn.
 namespace few {
-constexpr int FT = 64;                          // features a tile
 constexpr int MOST_ROWS = 128, MOST_STAGES = 11;
-constexpr int A_BYTES = 2 * FT * BK * 2;        // 16 KB
 constexpr int THREADS = 384;
 constexpr int SMEM_MOST = 200 * 1024;
-inline int stages_of(int n) { return std::min(MOST_STAGES, (SMEM_MOST - n * FT * 4) / (A_BYTES + n * 128)); }
-inline int smem_of(int n) { return stages_of(n) * (A_BYTES + n * 128) + n * FT * 4 + 1024 + 512; }
+constexpr int a_bytes(int ft) { return 2 * ft * BK * 2; }
+constexpr int exchange(int ft, int n) { return ft == 64 ? n * 64 * 4 : 0; }
+inline int stages_of(int ft, int n) {
+  return std::min(MOST_STAGES, (SMEM_MOST - exchange(ft, n)) / (a_bytes(ft) + n * 128));
+}
+inline int smem_of(int ft, int n) {
+  return stages_of(ft, n) * (a_bytes(ft) + n * 128) + exchange(ft, n) + 1024 + 512;
+}
 }  // namespace few
 
-template <int ACT, typename T>
+template <int ACT, typename T, int FT>
 __global__ void __launch_bounds__(few::THREADS, 1)
 few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ CUtensorMap tG,
-                const __grid_constant__ CUtensorMap tU, const Args a, const int n, const int stages) {
+                const __grid_constant__ CUtensorMap tU, const Args a, const int w, const int n,
+                const int stages) {
   using namespace few;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int stage_bytes = few::A_BYTES + n * 128;
-  float* ups = reinterpret_cast<float*>(smem + stages * stage_bytes);        // [n][FT]
-  uint64_t* full = reinterpret_cast<uint64_t*>(ups + n * FT);
+  constexpr int A_BYTES = a_bytes(FT);
+  const int stage_bytes = A_BYTES + n * 128;
+  float* ups = reinterpret_cast<float*>(smem + stages * stage_bytes);        // [n][FT], FT 64
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes + exchange(FT, n));
   uint64_t* empty = full + MOST_STAGES;
   uint64_t* acc_full = empty + MOST_STAGES;
   uint64_t* acc_empty = acc_full + NACC;
@@ -455,7 +466,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
     tma_prefetch_desc(&tG);
     tma_prefetch_desc(&tU);
   }
-  if (warp == 1) { tmem_alloc(tmem_slot, 2 * MOST_ROWS); tmem_relinquish(); }
+  if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -468,17 +479,17 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
       for (int kb = 0; kb < nk; ++kb) {
         if (!mbar_wait(&empty[s], phase, GWB_ERR_TIMEOUT_PRODUCER)) { ok = false; break; }
         uint8_t* sa = smem + s * stage_bytes;
-        mbar_arrive_expect_tx(&full[s], stage_bytes);
-        tma_load_2d(sa, &tG, &full[s], kb * BK, tile * FT);
-        tma_load_2d(sa + few::A_BYTES / 2, &tU, &full[s], kb * BK, tile * FT);
-        tma_load_2d(sa + few::A_BYTES, &tX, &full[s], kb * BK, 0);
+        mbar_arrive_expect_tx(&full[s], (2 * w + n) * 128);
+        tma_load_2d(sa, &tG, &full[s], kb * BK, tile * w);
+        tma_load_2d(sa + A_BYTES / 2, &tU, &full[s], kb * BK, tile * w);
+        tma_load_2d(sa + A_BYTES, &tX, &full[s], kb * BK, 0);
         if (++s == stages) { s = 0; phase ^= 1; }
       }
     if (!ok) land_copies();
   } else if (warp == 1 && lane == 0) {
     constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(n >> 3) << 17) |
-                           ((uint32_t)(2 * FT >> 4) << 24);
+                           (128u >> 4 << 24);
     int s = 0, phase = 0, lt = 0;
     bool ok = true;
     for (int tile = blockIdx.x; ok && tile < a.ntiles; tile += gridDim.x, ++lt) {
@@ -488,11 +499,15 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
       for (int kb = 0; kb < nk; ++kb) {
         if (!mbar_wait(&full[s], phase, GWB_ERR_TIMEOUT_MMA)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t ab = smem_u32(smem + s * stage_bytes), bb = ab + few::A_BYTES;
+        const uint32_t ab = smem_u32(smem + s * stage_bytes), bb = ab + A_BYTES;
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          mma_f16(tmem + b * MOST_ROWS, sdesc_k128(ab + 32 * k), sdesc_k128(bb + 32 * k), idesc,
-                  (kb > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < BK / 16; ++k) {
+          const uint32_t more = (kb > 0 || k > 0) ? 1u : 0u;
+          const uint64_t bd = sdesc_k128(bb + 32 * k);
+          mma_f16(tmem + b * 256, sdesc_k128(ab + 32 * k), bd, idesc, more);
+          if (FT == 128)
+            mma_f16(tmem + b * 256 + 128, sdesc_k128(ab + A_BYTES / 2 + 32 * k), bd, idesc, more);
+        }
         mma_commit(&empty[s]);
         if (++s == stages) { s = 0; phase ^= 1; }
       }
@@ -500,8 +515,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
     }
   } else if (warp >= 4) {
     const int q = warp & 3, half = (warp - 4) >> 2;
-    const int fl = 32 * (q & 1) + lane;                 // feature within the tile
-    // 16 columns (rows of x) at a time, halves in turn
+    const int fl = 32 * (FT == 64 ? q & 1 : q) + lane;  // feature within the tile
     const int chunks = n / 16;
     int lt = 0;
     bool ok = true;
@@ -509,30 +523,34 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
       const int b = lt & 1;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE));
       tc_fence_after();
-      const int f = tile * FT + fl;
-      const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + b * MOST_ROWS;
-      uint32_t v[16];
-      if (q >= 2) {
-        for (int c = half; c < chunks; c += 2) {
-          tmem_ld16(base + 16 * c, v);
-          tmem_wait_ld();
+      const int f = tile * w + fl;
+      const bool mine = fl < w && f < a.F;
+      const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + b * 256;
+      uint32_t v[16], vu[16];
+      if (FT == 64) {
+        if (q >= 2)
+          for (int c = half; c < chunks; c += 2) {
+            tmem_ld16(base + 16 * c, v);
+            tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) ups[(16 * c + j) * FT + fl] = __uint_as_float(v[j]);
-        }
+            for (int j = 0; j < 16; ++j) ups[(16 * c + j) * FT + fl] = __uint_as_float(v[j]);
+          }
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // ups is written
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");    // ups is written
-      if (q < 2) {
-        const float bg = a.bg && f < a.F ? to_f32<T>(static_cast<const T*>(a.bg)[f]) : 0.0f;
-        const float bu = a.bu && f < a.F ? to_f32<T>(static_cast<const T*>(a.bu)[f]) : 0.0f;
+      if (FT == 128 || q < 2) {
+        const float bg = a.bg && mine ? to_f32<T>(static_cast<const T*>(a.bg)[f]) : 0.0f;
+        const float bu = a.bu && mine ? to_f32<T>(static_cast<const T*>(a.bu)[f]) : 0.0f;
         for (int c = half; c < chunks; c += 2) {
           tmem_ld16(base + 16 * c, v);
+          if (FT == 128) tmem_ld16(base + 128 + 16 * c, vu);
           tmem_wait_ld();
           float h[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            h[j] = activation<ACT, false>(__uint_as_float(v[j]) + bg).act *
-                   (ups[(16 * c + j) * FT + fl] + bu);
-          if (f < a.F && ok)
+          for (int j = 0; j < 16; ++j) {
+            const float u = FT == 128 ? __uint_as_float(vu[j]) : ups[(16 * c + j) * FT + fl];
+            h[j] = activation<ACT, false>(__uint_as_float(v[j]) + bg).act * (u + bu);
+          }
+          if (mine && ok)
 #pragma unroll
             for (int j = 0; j < 16; ++j)
               if (16 * c + j < a.M)
@@ -540,14 +558,15 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
         }
       }
       tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");    // ups and the accumulator are read
+      if (FT == 64) asm volatile("bar.sync 1, 256;" ::: "memory");   // ups is read
+      __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[b]);
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 2 * MOST_ROWS);
+  if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
 // ------------------------------------------------- dg, du and bias gradients
@@ -705,21 +724,27 @@ int few_rows(const void* x, int64_t xs, const void* wg, const void* wu, Args a, 
   const int n = cdiv(a.M, 16) * 16;
   if (int rc = bind_context()) return rc;
   CUtensorMap tx, tg, tu;
+  const int sms = sm_count(), waves = cdiv(a.F, 128 * sms);
+  const int w = std::max(8, cdiv(cdiv(a.F, sms * waves), 8) * 8), ft = w > 64 ? 128 : 64;
   if (int rc = tmap16(&tx, x, bf, a.D, a.M, xs, n)) return rc;
-  if (int rc = tmap16(&tg, wg, bf, a.D, a.F, a.D, few::FT)) return rc;
-  if (int rc = tmap16(&tu, wu, bf, a.D, a.F, a.D, few::FT)) return rc;
-  a.ntiles = cdiv(a.F, few::FT);
+  if (int rc = tmap16(&tg, wg, bf, a.D, a.F, a.D, w)) return rc;
+  if (int rc = tmap16(&tu, wu, bf, a.D, a.F, a.D, w)) return rc;
+  a.ntiles = cdiv(a.F, w);
   const auto go = [&](auto kern) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few::smem_of(n)) !=
-        cudaSuccess)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             few::smem_of(ft, n)) != cudaSuccess)
       return (int)GWB_E_LAUNCH;
-    kern<<<std::min(a.ntiles, sm_count()), few::THREADS, few::smem_of(n), st>>>(
-        tx, tg, tu, a, n, few::stages_of(n));
+    kern<<<std::min(a.ntiles, sms), few::THREADS, few::smem_of(ft, n), st>>>(
+        tx, tg, tu, a, w, n, few::stages_of(ft, n));
     return launch_status();
   };
-  if (a.act == GWB_ACT_SILU) return go(few_rows_kernel<GWB_ACT_SILU, T>);
-  if (a.act == GWB_ACT_GELU) return go(few_rows_kernel<GWB_ACT_GELU, T>);
-  return go(few_rows_kernel<GWB_ACT_GELU_TANH, T>);
+  const auto wide = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    return ft == 128 ? go(few_rows_kernel<ACT, T, 128>) : go(few_rows_kernel<ACT, T, 64>);
+  };
+  if (a.act == GWB_ACT_SILU) return wide(std::integral_constant<int, GWB_ACT_SILU>{});
+  if (a.act == GWB_ACT_GELU) return wide(std::integral_constant<int, GWB_ACT_GELU>{});
+  return wide(std::integral_constant<int, GWB_ACT_GELU_TANH>{});
 }
 
 template <typename T>
