@@ -382,9 +382,9 @@ int gwb_gated_linear_keep(const void* x, int64_t x_stride, const void* w_gate, c
                           int activation, int dtype, void* h, void* kept, void* stream);
 int64_t gwb_gated_linear_kept(int64_t M, int64_t F, int dtype);
 
-/* Bytes of the 256-byte aligned scratch `work` of gwb_gated_linear_backward
- * (0 when a size is not positive). */
-int64_t gwb_gated_linear_backward_work(int64_t M, int64_t F);
+/* Bytes of the 256-byte aligned scratch `work` of gwb_gated_linear_backward on
+ * the current device (0 when a size is not positive). */
+int64_t gwb_gated_linear_backward_work(int64_t M, int64_t D, int64_t F);
 
 /* Gradients of gwb_gated_linear, each NULL when not wanted: dx [M, D],
  * dw_gate / dw_up [F, D], db_gate / db_up [F], from dh [M, F] (row stride

@@ -486,7 +486,8 @@ static int gated_sizes(int64_t M, int64_t D, int64_t F, int activation, int dtyp
   if (!fits_int(M) || !fits_int(D) || !fits_int(F) || D == 0 || F == 0 || D % 8 || F % 8)
     return GWB_E_SHAPE;
   // tile counts are 32-bit
-  if ((M / 128 + 1) * (F / 128 + 1) > 0x7fffffff || (F / 64 + 2) * (D / 256 + 1) > 0x7fffffff)
+  if ((M / 128 + 1) * (F / 128 + 1) > 0x7fffffff || (F / 64 + 2) * (D / 256 + 1) > 0x7ffffff ||
+      (M / 256 + 1) * (D / 256 + 1) > 0x7ffffff)
     return GWB_E_CAPACITY;
   if (activation < GWB_ACT_SILU || activation > GWB_ACT_GELU_TANH) return GWB_E_SHAPE;
   return dtype == GWB_BF16 || dtype == GWB_F16 ? GWB_SUCCESS : GWB_E_SHAPE;
@@ -525,9 +526,9 @@ int64_t gwb_gated_linear_kept(int64_t M, int64_t F, int dtype) {
   return dtype == GWB_BF16 || dtype == GWB_F16 ? gwb::gated_kept_bytes(M, F, dtype) : 0;
 }
 
-int64_t gwb_gated_linear_backward_work(int64_t M, int64_t F) {
-  if (!fits_int(M) || !fits_int(F) || M == 0 || F == 0) return 0;
-  return gwb::gated_backward_work((int)M, (int)F);
+int64_t gwb_gated_linear_backward_work(int64_t M, int64_t D, int64_t F) {
+  if (!fits_int(M) || !fits_int(D) || !fits_int(F) || M == 0 || D == 0 || F == 0) return 0;
+  return gwb::gated_backward_work((int)M, (int)D, (int)F);
 }
 
 int gwb_gated_linear_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,

@@ -45,12 +45,26 @@ enum Mode { FORWARD, SAVE, DGATE, DX, DW };
 // where a CTA alone needs 48 KB for a 128 x 256 tile, and a third less is
 // copied and read from shared memory per operation.
 constexpr int BM = 128, BN = 256, BK = 64;      // BK elements = one 128-byte swizzle row
-constexpr int STAGES = 6;
 constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / 2 * BK * 2;   // of one CTA
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int MN_BOX = 64 * BK * 2;             // a 64 (MN) x 64 (K) box of an MN-major operand
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
 constexpr int THREADS = 384, EPI0 = 4, EPI_WARPS = 8;
+constexpr int PATCH = 32 * 128;                 // an epilogue warp's 32 rows of 128 bytes
+// Stages, and the epilogue's patches where an epilogue has them (SAVE, and a
+// product whose second template argument says so): what is left of the 256 KB
+// is the L1 that direct stores go through.
+template <int MODE, int ACT> constexpr bool patched() {
+  return MODE == SAVE || ((MODE == DX || MODE == DW) && ACT);
+}
+template <int MODE, int ACT> constexpr int stages() { return patched<MODE, ACT>() ? 5 : 6; }
+template <int MODE, int ACT> constexpr int smem_bytes() {
+  return stages<MODE, ACT>() * STAGE_BYTES + (patched<MODE, ACT>() ? EPI_WARPS * PATCH : 0) + 1024 +
+         256;
+}
+// Short items leave the epilogue no k-loop to hide behind: whole lines then.
+// With 48 k-blocks or more the patches' shared memory costs more than it saves
+// (dx and dw of 4608 x 3072 -> 12288: 1055 us with, 1037 without).
+constexpr int PATCH_K = 48;
 constexpr int NACC = 2, TMEM_COLS = NACC * BN;
 // Tiles are walked in groups of eight row tiles: the 74 pairs at work then read
 // about 8 row tiles and 9 column tiles, near the fewest operand bytes.
@@ -63,6 +77,9 @@ struct Args {
   int M, D, F, act;
   void* kept; float* kept_scale;      // SAVE: a and b, planes [2][M][F], and their scales
   int tiles_m, tiles_n, half0, ntiles;
+  // DX, DW with few tiles: each tile's K is split into `parts` of `part_k`
+  // k-blocks, and part p's f32 tile goes to partial + p * part_stride
+  int parts, part_k; float* partial; int64_t part_stride;
 };
 
 // The type a and b are kept in, and whether each row's 64 columns have a scale.
@@ -168,15 +185,43 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
   *reinterpret_cast<uint4*>(p) = round8<T>(f);
 }
 
+// The kept planes and the gradients leave by way of shared memory, 128 bytes of
+// each of a warp's 32 rows at a time: a lane holds one row, and storing it
+// directly touches 32 lines with every instruction (7473 x 304 -> 6984 f16 with
+// its f32 planes: 325 us directly, 185 so; the gradients of 128 rows of 3072 ->
+// 12288: 142 and 101). h is stored directly all the same: the detour cost it
+// more than the lines did (41 against 47 us at 1531 x 1416 -> 3880). 16-byte
+// pieces are swizzled by row, so both sides are free of bank conflicts.
+__device__ __forceinline__ void patch_put(uint8_t* patch, int lane, int piece, uint4 v) {
+  *reinterpret_cast<uint4*>(patch + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
+}
+// rows and columns that exist; K elements of 16 or 32 bits
+template <typename K>
+__device__ __forceinline__ void patch_store(const uint8_t* patch, int lane, K* dst, int64_t ld,
+                                            int rows, int cols) {
+  constexpr int N = 16 / (int)sizeof(K);
+  __syncwarp();
+  const int piece = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3);
+    const uint4 v = *reinterpret_cast<const uint4*>(patch + r * 128 + ((piece ^ (r & 7)) << 4));
+    if (r < rows && piece * N < cols) *reinterpret_cast<uint4*>(dst + r * ld + piece * N) = v;
+  }
+  __syncwarp();
+}
+
 template <int MODE, int ACT, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
              const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1,
              const Args a) {
   constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW, PROJ = !B_MN;
+  constexpr bool PATCHED = patched<MODE, ACT>();
+  constexpr int STAGES = stages<MODE, ACT>(), PATCHES = PATCHED ? EPI_WARPS * PATCH : 0;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);   // the leader's count
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + PATCHES);   // the leader's count
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + NACC;                                       // the leader's count
@@ -214,10 +259,12 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
       int it = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < a.ntiles; tile += pairs) {
-        const Tile t = tile_of<MODE>(a, tile);
+        const Tile t = tile_of<MODE>(a, PROJ ? tile : tile / a.parts);
         const int m0 = t.m0 + (int)rank * BM;         // this CTA's rows of A
         const int bn = (int)rank * (BN / 2);          // its part of B's rows
-        for (int kb = 0; kb < nk; ++kb, ++it) {
+        const int k0b = PROJ ? 0 : tile % a.parts * a.part_k;
+        const int k1b = PROJ ? nk : min(nk, k0b + a.part_k);
+        for (int kb = k0b; kb < k1b; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, GWB_ERR_TIMEOUT_PRODUCER)) {
             ok = false;
@@ -261,7 +308,9 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
         if (!mbar_wait(&acc_empty[b], ((lt >> 1) & 1) ^ 1, GWB_ERR_TIMEOUT_MMA)) break;
         tc_fence_after();
         const uint32_t d = tmem + b * BN;
-        for (int kb = 0; kb < nk; ++kb, ++it) {
+        const int k0b = PROJ ? 0 : tile % a.parts * a.part_k;
+        const int k1b = PROJ ? nk : min(nk, k0b + a.part_k);
+        for (int kb = k0b; kb < k1b; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&full[s], (it / STAGES) & 1, GWB_ERR_TIMEOUT_MMA)) { ok = false; break; }
           tc_fence_after();
@@ -270,7 +319,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
           for (int k = 0; k < BK / 16; ++k)
             mma_f16_pair(d, A_MN ? sdesc_mn128(ab + 2048 * k, MN_BOX) : sdesc_k128(ab + 32 * k),
                          B_MN ? sdesc_mn128(bb + 2048 * k, MN_BOX) : sdesc_k128(bb + 32 * k), idesc,
-                         (kb > 0 || k > 0) ? 1u : 0u);
+                         (kb > k0b || k > 0) ? 1u : 0u);
           mma_commit_pair(&empty[s]);
         }
         if (ok) mma_commit_pair(&acc_full[b]);
@@ -279,17 +328,17 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
   } else {
     regs_inc<232>();
     const int q = warp & 3, side = (warp - EPI0) >> 2;
+    uint8_t* patch = smem + STAGES * STAGE_BYTES + (warp - EPI0) * PATCH;
     int lt = 0;
     for (int tile = pair; tile < a.ntiles; tile += pairs, ++lt) {
-      Tile t = tile_of<MODE>(a, tile);
-      t.m0 += (int)rank * BM;
+      const Tile t = tile_of<MODE>(a, PROJ ? tile : tile / a.parts);
       const int b = lt & 1;
       if (!mbar_wait(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
       __syncwarp();
       tc_fence_after();
       uint32_t v[128];
       const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + b * BN;
-      const int row = t.m0 + 32 * q + lane;
+      const int row0 = t.m0 + (int)rank * BM + 32 * q, row = row0 + lane;    // the lane's row
       if constexpr (PROJ) {
         // v[0..63] gate and v[64..127] up of columns n0 + 64 side ..
         tmem_ld32(base + 64 * side, v);
@@ -305,12 +354,13 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[b], 0));
       if constexpr (PROJ) {
-        if (row >= a.M) continue;
-        const int n0 = t.n0 + 64 * side;
+        const int n0 = t.n0 + 64 * side, rows = a.M - row0, cols = a.F - n0;
+        if (rows <= 0 || cols <= 0) continue;
+        if (MODE != SAVE && row >= a.M) continue;      // SAVE's lanes store for each other
         float amax_a = 0.0f, amax_b = 0.0f;
 #pragma unroll
         for (int c = 0; c < 64; c += 8) {
-          if (n0 + c >= a.F) break;
+          if (c >= cols) break;
           float g[8], u[8], p[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -327,16 +377,15 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
 #pragma unroll
             for (int j = 0; j < 8; ++j) u[j] += p[j];
           }
-          const size_t at = (size_t)row * a.F + n0 + c;
-          float o0[8], o1[8];
+          float o[8];
           if constexpr (MODE == FORWARD) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o0[j] = activation<ACT, false>(g[j]).act * u[j];
+            for (int j = 0; j < 8; ++j) o[j] = activation<ACT, false>(g[j]).act * u[j];
           } else if constexpr (MODE == SAVE) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const ActValue f = activation<ACT, true>(g[j]);
-              o0[j] = f.act * u[j];
+              o[j] = f.act * u[j];
               const float fa = u[j] * f.slope;
               v[c + j] = __float_as_uint(fa);
               v[64 + c + j] = __float_as_uint(f.act);
@@ -350,56 +399,89 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const ActValue f = activation<ACT, true>(g[j]);
-              o0[j] = p[j] * u[j] * f.slope;
-              o1[j] = p[j] * f.act;
+              o[j] = p[j] * u[j] * f.slope;
+              p[j] *= f.act;
             }
-            store8(static_cast<T*>(a.o1) + at, o1);
+            store8(static_cast<T*>(a.o1) + (size_t)row * a.F + n0 + c, p);
           }
-          store8(static_cast<T*>(a.o0) + at, o0);
+          if (MODE != SAVE || row < a.M)
+            store8(static_cast<T*>(a.o0) + (size_t)row * a.F + n0 + c, o);
         }
         if constexpr (MODE == SAVE) {
           using K = typename Kept<T>::type;
+          // columns [0, 64) of v from `first` on, times s, to dst
+          const auto put = [&](K* dst, int first, float s) {
+            constexpr int N = 16 / (int)sizeof(K), WIDE = 8 * N;       // columns a patch holds
+#pragma unroll
+            for (int c0 = 0; c0 < 64; c0 += WIDE) {
+#pragma unroll
+              for (int c = 0; c < WIDE; c += N) {
+                uint4 w;
+                if constexpr (sizeof(K) == 2) {
+                  float o[8];
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(v[first + c0 + c + j]) * s;
+                  w = round8<K>(o);
+                } else {
+                  w = make_uint4(v[first + c0 + c], v[first + c0 + c + 1], v[first + c0 + c + 2],
+                                 v[first + c0 + c + 3]);
+                }
+                patch_put(patch, lane, c / N, w);
+              }
+              patch_store(patch, lane, dst + c0, a.F, rows, cols - c0);
+            }
+          };
           const float sa = Kept<T>::scaled ? kept_scale_of(amax_a) : 1.0f;
           const float sb = Kept<T>::scaled ? kept_scale_of(amax_b) : 1.0f;
-          if (Kept<T>::scaled && n0 < a.F) {
+          if (Kept<T>::scaled && row < a.M) {
             const int groups = (a.F + 63) / 64;
             a.kept_scale[(size_t)row * groups + n0 / 64] = sa;
             a.kept_scale[(size_t)(a.M + row) * groups + n0 / 64] = sb;
           }
-          K* ka = static_cast<K*>(a.kept) + (size_t)row * a.F + n0;
-          K* kb = ka + (size_t)a.M * a.F;
-#pragma unroll
-          for (int c = 0; c < 64; c += 8) {
-            if (n0 + c >= a.F) break;
-            float oa[8], ob[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              oa[j] = __uint_as_float(v[c + j]) * sa;
-              ob[j] = __uint_as_float(v[64 + c + j]) * sb;
-            }
-            if constexpr (sizeof(K) == 2) {
-              store8(ka + c, oa);
-              store8(kb + c, ob);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; j += 4) {
-                *reinterpret_cast<float4*>(ka + c + j) = make_float4(oa[j], oa[j + 1], oa[j + 2], oa[j + 3]);
-                *reinterpret_cast<float4*>(kb + c + j) = make_float4(ob[j], ob[j + 1], ob[j + 2], ob[j + 3]);
-              }
-            }
-          }
+          K* ka = static_cast<K*>(a.kept) + (size_t)row0 * a.F + n0;
+          put(ka, 0, sa);
+          put(ka + (size_t)a.M * a.F, 64, sb);
         }
       } else {
-        if (row >= (MODE == DX ? a.M : a.F)) continue;
-        T* out = static_cast<T*>(t.half ? a.o1 : a.o0) + (size_t)row * a.D;
-        const int n0 = t.n0 + 128 * side;
+        const int total = MODE == DX ? a.M : a.F, n0 = t.n0 + 128 * side;
+        const int rows = total - row0, cols = a.D - n0;
+        if (rows <= 0 || cols <= 0) continue;
+        if constexpr (!PATCHED) {
+          if (row >= total) continue;
+          T* dst = static_cast<T*>(t.half ? a.o1 : a.o0) + (size_t)row * a.D + n0;
 #pragma unroll
-        for (int c = 0; c < 128; c += 8) {
-          if (n0 + c >= a.D) break;
-          float o[8];
+          for (int c = 0; c < 128; c += 8) {
+            if (c >= cols) break;
+            float o[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(v[c + j]);
-          store8(out + n0 + c, o);
+            for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(v[c + j]);
+            store8(dst + c, o);
+          }
+        } else if (a.parts > 1) {
+          // this part's f32 tile; DW's two gradients are rows of one matrix
+          float* dst = a.partial + (int64_t)(tile % a.parts) * a.part_stride +
+                       ((int64_t)(t.half - a.half0) * a.F + row0) * a.D + n0;
+#pragma unroll
+          for (int c0 = 0; c0 < 128; c0 += 32) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              patch_put(patch, lane, c / 4,
+                        make_uint4(v[c0 + c], v[c0 + c + 1], v[c0 + c + 2], v[c0 + c + 3]));
+            patch_store(patch, lane, dst + c0, a.D, rows, cols - c0);
+          }
+        } else {
+          T* dst = static_cast<T*>(t.half ? a.o1 : a.o0) + (size_t)row0 * a.D + n0;
+#pragma unroll
+          for (int c0 = 0; c0 < 128; c0 += 64) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 8) {
+              float o[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(v[c0 + c + j]);
+              patch_put(patch, lane, c / 8, round8<T>(o));
+            }
+            patch_store(patch, lane, dst + c0, a.D, rows, cols - c0);
+          }
         }
       }
     }
@@ -648,6 +730,23 @@ gradients_kernel(const T* __restrict__ dh, int64_t dhs, const void* __restrict__
   }
 }
 
+// Sums a split product's parts in order: out0 [rows0][D], then out1.
+template <typename T>
+__global__ void __launch_bounds__(256)
+parts_join_kernel(const float* __restrict__ partial, int parts, int64_t stride, int64_t n0,
+                  int64_t n, T* __restrict__ out0, T* __restrict__ out1) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (i >= n) return;
+  float t[8] = {};
+  for (int p = 0; p < parts; ++p) {
+    const float4* src = reinterpret_cast<const float4*>(partial + p * stride + i);
+    const float4 a = __ldcs(src), b = __ldcs(src + 1);
+    t[0] += a.x; t[1] += a.y; t[2] += a.z; t[3] += a.w;
+    t[4] += b.x; t[5] += b.y; t[6] += b.z; t[7] += b.w;
+  }
+  store8(i < n0 ? out0 + i : out1 + (i - n0), t);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256)
 column_join_kernel(const float* __restrict__ partial, int chunks, int F, T* dbg, T* dbu) {
@@ -685,13 +784,15 @@ int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0,
   if (cudaGetDevice(&dev) != cudaSuccess) return GWB_E_LAUNCH;
   const uint64_t bit = 1ull << (dev & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) !=
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             smem_bytes<MODE, ACT>()) !=
         cudaSuccess)
       return GWB_E_LAUNCH;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const int pairs = sm_count() / 2;
-  kern<<<2 * (a.ntiles < pairs ? a.ntiles : pairs), THREADS, SMEM_BYTES, st>>>(a0, a1, b0, b1, a);
+  kern<<<2 * (a.ntiles < pairs ? a.ntiles : pairs), THREADS, smem_bytes<MODE, ACT>(), st>>>(a0, a1, b0,
+                                                                                   b1, a);
   return launch_status();
 }
 
@@ -778,6 +879,48 @@ inline int bias_chunks(int M, int F) {
   return want < most ? (want > 0 ? want : 1) : (most > 0 ? most : 1);
 }
 
+// How a product of `tiles` tiles of nk k-blocks is split along K: the parts (at
+// most 16, of eight k-blocks at least) for which the pairs of multiprocessors
+// finish first, counting 512 cycles a k-block, 3000 an item, and the parts'
+// f32 values written and read at 3400 bytes a cycle. One part wherever there
+// are tiles enough; at 1000 x 256 x 8192, dx has 4 tiles of 256 k-blocks and 74
+// pairs to work on them: 99 us in one part, 20 in 16.
+struct Split { int parts, part_k; };
+inline Split split_of(int64_t tiles, int nk, int64_t elements) {
+  const int64_t pairs = sm_count() / 2;
+  Split best{1, nk};
+  int64_t cost = -1;
+  for (int parts = 1; parts <= 16 && (parts == 1 || nk / parts >= 8); ++parts) {
+    const int per = cdiv(nk, parts);
+    if (cdiv(nk, per) != parts) continue;
+    int64_t c = (tiles * parts + pairs - 1) / pairs * (per * 512 + 3000);
+    if (parts > 1) c += elements * 8 * parts / 3400 + 6000;
+    if (cost < 0 || c < cost) { cost = c; best = {parts, per}; }
+  }
+  return best;
+}
+inline Split split_dx(int M, int D, int F) {
+  return split_of((int64_t)cdiv(M, 2 * BM) * cdiv(D, BN), 2 * cdiv(F, BK), (int64_t)M * D);
+}
+inline Split split_dw(int M, int D, int F, int halves) {
+  return split_of((int64_t)halves * cdiv(F, 2 * BM) * cdiv(D, BN), cdiv(M, BK),
+                  (int64_t)halves * F * D);
+}
+inline int64_t partial_bytes(const Split& s, int64_t elements) {
+  return s.parts > 1 ? s.parts * elements * 4 : 0;
+}
+
+inline int64_t bias_bytes(int M, int F) {
+  return ((int64_t)2 * bias_chunks(M, F) * F * 4 + 255) / 256 * 256;
+}
+
+template <typename T>
+int join(const Args& a, int64_t n0, int64_t n, cudaStream_t st) {
+  parts_join_kernel<T><<<(unsigned)((n / 8 + 255) / 256), 256, 0, st>>>(
+      a.partial, a.parts, a.part_stride, n0, n, static_cast<T*>(a.o0), static_cast<T*>(a.o1));
+  return launch_status();
+}
+
 template <typename T>
 int backward(const GatedBackward& w, cudaStream_t st) {
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
@@ -787,6 +930,7 @@ int backward(const GatedBackward& w, cudaStream_t st) {
   void* dg = p;
   void* du = p + plane;
   float* partial = reinterpret_cast<float*>(p + 2 * plane);
+  float* parts = reinterpret_cast<float*>(p + 2 * plane + bias_bytes(M, F));
   Args a{};
   a.bg = w.bg; a.bu = w.bu; a.dh = w.dh; a.dhs = w.dhs; a.o0 = dg; a.o1 = du;
   a.M = M; a.D = D; a.F = F; a.act = w.act;
@@ -812,8 +956,16 @@ int backward(const GatedBackward& w, cudaStream_t st) {
     c.o0 = w.dx;
     c.tiles_m = cdiv(M, 2 * BM);
     c.tiles_n = cdiv(D, BN);
-    c.ntiles = c.tiles_m * c.tiles_n;
-    if (int rc = launch<DX, 0, T>(ag, au, bgm, bum, c, st)) return rc;
+    const Split sp = split_dx(M, D, F);
+    c.parts = sp.parts; c.part_k = sp.part_k;
+    c.partial = parts; c.part_stride = (int64_t)M * D;
+    c.ntiles = c.tiles_m * c.tiles_n * c.parts;
+    const bool patch = c.parts > 1 || c.part_k < PATCH_K;
+    if (int rc = patch ? launch<DX, 1, T>(ag, au, bgm, bum, c, st)
+                       : launch<DX, 0, T>(ag, au, bgm, bum, c, st))
+      return rc;
+    if (c.parts > 1)
+      if (int rc = join<T>(c, c.part_stride, c.part_stride, st)) return rc;
   }
   if (w.dwg || w.dwu) {
     CUtensorMap ag, au, bx;
@@ -826,8 +978,17 @@ int backward(const GatedBackward& w, cudaStream_t st) {
     c.half0 = w.dwg ? 0 : 1;
     c.tiles_m = cdiv(F, 2 * BM) * (w.dwg && w.dwu ? 2 : 1);
     c.tiles_n = cdiv(D, BN);
-    c.ntiles = c.tiles_m * c.tiles_n;
-    if (int rc = launch<DW, 0, T>(ag, au, bx, bx, c, st)) return rc;
+    const int halves = w.dwg && w.dwu ? 2 : 1;
+    const Split sp = split_dw(M, D, F, halves);
+    c.parts = sp.parts; c.part_k = sp.part_k;
+    c.partial = parts; c.part_stride = (int64_t)halves * F * D;
+    c.ntiles = c.tiles_m * c.tiles_n * c.parts;
+    const bool patch = c.parts > 1 || c.part_k < PATCH_K;
+    if (int rc = patch ? launch<DW, 1, T>(ag, au, bx, bx, c, st)
+                       : launch<DW, 0, T>(ag, au, bx, bx, c, st))
+      return rc;
+    if (c.parts > 1)
+      if (int rc = join<T>(c, w.dwg ? (int64_t)F * D : 0, c.part_stride, st)) return rc;
   }
   if (bias) {
     if (!w.kept) {
@@ -845,9 +1006,13 @@ int backward(const GatedBackward& w, cudaStream_t st) {
 
 }  // namespace gated
 
-int64_t gated_backward_work(int M, int F) {
+int64_t gated_backward_work(int M, int D, int F) {
+  using namespace gated;
   const int64_t plane = ((int64_t)M * F * 2 + 255) / 256 * 256;
-  return 2 * plane + (int64_t)2 * gated::bias_chunks(M, F) * F * 4;
+  const int64_t dx = partial_bytes(split_dx(M, D, F), (int64_t)M * D);
+  const int64_t dw2 = partial_bytes(split_dw(M, D, F, 2), (int64_t)2 * F * D);
+  const int64_t dw1 = partial_bytes(split_dw(M, D, F, 1), (int64_t)F * D);
+  return 2 * plane + bias_bytes(M, F) + std::max(dx, std::max(dw1, dw2));
 }
 
 int64_t gated_kept_bytes(int64_t M, int64_t F, int dtype) {

@@ -614,7 +614,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_linear_backward_cuda(
   };
   Tensor dx = out(mask[0], x.sizes()), dwg = out(mask[1], wg.sizes()), dwu = out(mask[2], wu.sizes());
   Tensor dbg = out(mask[3], {g.f}), dbu = out(mask[4], {g.f});
-  Tensor work = at::empty({gwb_gated_linear_backward_work(g.rows, g.f)},
+  Tensor work = at::empty({gwb_gated_linear_backward_work(g.rows, g.d, g.f)},
                           x.options().dtype(at::kByte));
   const auto at_ = [](bool on, Tensor& t) { return on ? t.data_ptr() : nullptr; };
   check_status(gwb_gated_linear_backward(

@@ -90,7 +90,7 @@ _SIGNATURES = {
     "gwb_gated_linear_keep": [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64,
                               c_i64, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "gwb_gated_linear_kept": [c_i64, c_i64, c_int],
-    "gwb_gated_linear_backward_work": [c_i64, c_i64],
+    "gwb_gated_linear_backward_work": [c_i64, c_i64, c_i64],
     "gwb_gated_linear_backward": [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_i64, c_i64, c_i64, c_int, c_int, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],

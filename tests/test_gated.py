@@ -99,6 +99,18 @@ def test_activations_and_biases(cuda_ready, recompute, m, act, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,d,f", [(40, 72, 4104), (1000, 256, 2600), (3000, 96, 136), (2100, 8, 264)])
+def test_split_products(cuda_ready, m, d, f, dtype):
+    """Gradients of few tiles and a long sum, which is split and joined: both
+    weights', one weight's, and x's."""
+    p = make(m, d, f, dtype, bias=m == 1000)
+    verify(p, "silu", *run(p))
+    for names in (["w_up"], ["w_gate"], ["x"]):
+        verify(p, "silu", *run(p, names=names))
+
+
+@pytest.mark.gpu
 def test_many_tiles(cuda_ready):
     """More tiles than multiprocessors, so the persistent walk wraps."""
     p = make(1100, 520, 2600, torch.bfloat16, bias=True)
@@ -325,5 +337,7 @@ def test_refusals_on_the_cpu():
     for kw in ({"d": 0}, {"f": 0}, {"d": 12}, {"f": 9}, {"m": -1}, {"act": 3}, {"act": -1}, {"dtype": 0},
                {}):
         assert call(**kw) == 1, kw
-    assert lib.gwb_gated_linear_backward_work(0, 8) == 0
-    assert lib.gwb_gated_linear_backward_work(3, 8) == 2 * 256 + 2 * 8 * 4
+    assert lib.gwb_gated_linear_backward_work(0, 8, 8) == 0
+    assert lib.gwb_gated_linear_backward_work(3, 8, 8) == 2 * 256 + 256
+    assert lib.gwb_gated_linear_kept(3, 40, 1) == 3 * 40 * 4 + 3 * 8
+    assert lib.gwb_gated_linear_kept(3, 40, 2) == 3 * 40 * 8 and lib.gwb_gated_linear_kept(3, 40, 0) == 0
