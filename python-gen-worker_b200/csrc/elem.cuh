@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -115,6 +117,20 @@ __device__ __forceinline__ uint4 repack(const F2 (&o)[Pairs<T>::N]) {
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
   }
+}
+
+// Lets a kernel use up to `most` bytes of dynamic shared memory, asked of the
+// driver once per device (a call costs more than a launch). `ready` belongs to
+// the kernel.
+inline bool allow_smem(const void* kern, std::atomic<uint64_t>& ready, int most) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (ready.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+    return false;
+  ready.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 // Host-side status of a launch: clears the sticky-free error of this call only.

@@ -778,18 +778,9 @@ template <int MODE, int ACT, typename T>
 int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0,
            const CUtensorMap& b1, Args a, cudaStream_t st) {
   auto kern = gated_kernel<MODE, ACT, T>;
-  // the shared-memory limit is a property of the function on each device
   static std::atomic<uint64_t> ready{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return GWB_E_LAUNCH;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             smem_bytes<MODE, ACT>()) !=
-        cudaSuccess)
-      return GWB_E_LAUNCH;
-    ready.fetch_or(bit, std::memory_order_relaxed);
-  }
+  if (!allow_smem(reinterpret_cast<const void*>(kern), ready, smem_bytes<MODE, ACT>()))
+    return GWB_E_LAUNCH;
   const int pairs = sm_count() / 2;
   kern<<<2 * (a.ntiles < pairs ? a.ntiles : pairs), THREADS, smem_bytes<MODE, ACT>(), st>>>(a0, a1, b0,
                                                                                    b1, a);
@@ -831,21 +822,22 @@ int few_rows(const void* x, int64_t xs, const void* wg, const void* wu, Args a, 
   if (int rc = tmap16(&tg, wg, bf, a.D, a.F, a.D, w)) return rc;
   if (int rc = tmap16(&tu, wu, bf, a.D, a.F, a.D, w)) return rc;
   a.ntiles = cdiv(a.F, w);
-  const auto go = [&](auto kern) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             few::smem_of(ft, n)) != cudaSuccess)
+  const auto wide = [&](auto act, auto feats) {
+    auto kern = few_rows_kernel<decltype(act)::value, T, decltype(feats)::value>;
+    static std::atomic<uint64_t> ready{0};
+    if (!allow_smem(reinterpret_cast<const void*>(kern), ready, few::SMEM_MOST + 1024 + 512))
       return (int)GWB_E_LAUNCH;
     kern<<<std::min(a.ntiles, sms), few::THREADS, few::smem_of(ft, n), st>>>(
         tx, tg, tu, a, w, n, few::stages_of(ft, n));
     return launch_status();
   };
-  const auto wide = [&](auto act) {
-    constexpr int ACT = decltype(act)::value;
-    return ft == 128 ? go(few_rows_kernel<ACT, T, 128>) : go(few_rows_kernel<ACT, T, 64>);
+  const auto go = [&](auto act) {
+    return ft == 128 ? wide(act, std::integral_constant<int, 128>{})
+                     : wide(act, std::integral_constant<int, 64>{});
   };
-  if (a.act == GWB_ACT_SILU) return wide(std::integral_constant<int, GWB_ACT_SILU>{});
-  if (a.act == GWB_ACT_GELU) return wide(std::integral_constant<int, GWB_ACT_GELU>{});
-  return wide(std::integral_constant<int, GWB_ACT_GELU_TANH>{});
+  if (a.act == GWB_ACT_SILU) return go(std::integral_constant<int, GWB_ACT_SILU>{});
+  if (a.act == GWB_ACT_GELU) return go(std::integral_constant<int, GWB_ACT_GELU>{});
+  return go(std::integral_constant<int, GWB_ACT_GELU_TANH>{});
 }
 
 template <typename T>

@@ -169,6 +169,7 @@ struct FwdPlan {
   int chunks;                    // CTAs a sample
   int64_t chunk_rows;            // rows of one, a multiple of slot_rows
   int slot_rows, stages;         // rows a copy brings, slots a warp
+  int warps;                     // warps that take rows; any others help with g and h
   uint32_t slot_bytes;
 };
 
@@ -185,7 +186,7 @@ forward_kernel(const FwdArgs a, const FwdPlan p) {
   constexpr int VEC = 16 / (int)sizeof(T), P = Pairs<T>::N, C = E / VEC, G = 32 / L;
   constexpr int SURE = LO / VEC;                         // vectors that every lane has
   extern __shared__ __align__(16) uint8_t smem[];
-  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warps = p.warps, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int l = lane % L, sub = lane / L;
   const int pd = (a.D + 3) & ~3;
   float* gs = reinterpret_cast<float*>(smem);            // [pd] g, [pd] h
@@ -212,20 +213,32 @@ forward_kernel(const FwdArgs a, const FwdPlan p) {
     mbar_arrive_expect_tx(&full[s % p.stages], bytes);
     if (bytes) bulk_load(dst, span_of(src, n).from, bytes, &full[s % p.stages]);
   };
-  if (lane == 0) {
+  if (lane == 0 && warp < warps) {
     for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
     for (int s = 0; s < p.stages && s < steps; ++s) fill(s);
   }
   const bool params = a.w.p || a.b.p || a.s.p || a.t.p;
   if (params)
-    for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
-      // VECTOR: four columns of a vector a plane, so that the lanes' 16-byte
-      // reads adjoin (a vector's eight in a row would share banks two by two)
-      const int at = VECTOR ? c % VEC / 4 * (a.D / (VEC / 4)) + c / VEC * 4 + c % 4 : c;
-      combine<T>(a.w, a.b, a.s, a.t, smp, c, gs[at], hs[at]);
+    for (int c0 = threadIdx.x; c0 < a.D; c0 += 4 * blockDim.x) {
+      // four columns' loads in flight together
+      float g[4], h[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = c0 + k * (int)blockDim.x;
+        if (c < a.D) combine<T>(a.w, a.b, a.s, a.t, smp, c, g[k], h[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // VECTOR: four columns of a vector a plane, so that the lanes' 16-byte
+        // reads adjoin (a vector's eight in a row would share banks two by two)
+        const int c = c0 + k * (int)blockDim.x;
+        const int at = VECTOR ? c % VEC / 4 * (a.D / (VEC / 4)) + c / VEC * 4 + c % 4 : c;
+        if (c < a.D) { gs[at] = g[k]; hs[at] = h[k]; }
+      }
     }
   __syncthreads();
+  if (warp >= warps) return;
   const float inv_d = 1.0f / (float)a.D;
   const int nvec = a.D / VEC;
   T* y = static_cast<T*>(a.y);
@@ -939,10 +952,12 @@ int forward_l(FwdArgs a, cudaStream_t st) {
   if (blocks > 0x7fffffff) return GWB_E_CAPACITY;
   const size_t smem = ((2 * ((a.D + 3) & ~3) * 4 + warps * p.stages * 8 + 15) & ~15) +
                       (size_t)warps * p.stages * p.slot_bytes;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-      cudaSuccess)
-    return GWB_E_LAUNCH;
-  kern<<<(unsigned)blocks, warps * 32, smem, st>>>(a, p);
+  static std::atomic<uint64_t> ready{0};
+  if (!allow_smem(reinterpret_cast<const void*>(kern), ready, 225 * 1024)) return GWB_E_LAUNCH;
+  // a CTA of few rows has many columns of g and h for few warps
+  const bool params = a.w.p || a.b.p || mod;
+  p.warps = warps;
+  kern<<<(unsigned)blocks, 32 * (params ? std::max(warps, 8) : warps), smem, st>>>(a, p);
   return launch_status();
 }
 
@@ -998,9 +1013,8 @@ int backward_staged_e(const BwdArgs& a, int64_t blocks, int64_t rows, int th, cu
   p.stages = std::max(3, std::min(8, (220 * 1024 / per_sm - 2048) / slot));
   const size_t smem = (size_t)p.stages * slot;
   if (smem > 226 * 1024) return GWB_E_SHAPE;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-      cudaSuccess)
-    return GWB_E_LAUNCH;
+  static std::atomic<uint64_t> ready{0};
+  if (!allow_smem(reinterpret_cast<const void*>(kern), ready, 226 * 1024)) return GWB_E_LAUNCH;
   kern<<<(unsigned)blocks, th + 32, smem, st>>>(a, p);
   return launch_status();
 }
