@@ -1,0 +1,197 @@
+"""The block operators as a transformer block runs them, beside the quantised
+linears: modulation -> norm -> quantised qkv -> rotary -> attention -> quantised
+out, norm -> gated projections -> quantised down; eager, captured and as a
+training step."""
+
+import pytest
+import torch
+
+from block_reference import ROTARY_COUNT, U, check, gated64, gated_magnitudes, norm64, norm_magnitudes, rotary64
+
+DIM, HEADS, HEAD, HIDDEN, TOKENS, BATCH = 512, 4, 128, 1024, 97, 2
+
+
+def build():
+    """One block's modules on the GPU, from seeded dense weights."""
+    import gen_worker_b200 as gw
+    from gen_worker_b200.awq import AwqPackedLinear
+
+    torch.manual_seed(5)
+
+    def linear(i, o):
+        lin = torch.nn.Linear(i, o, device="cuda", dtype=torch.bfloat16)
+        with torch.no_grad():
+            lin.weight.normal_(0, i ** -0.5)
+            lin.bias.normal_(0, 0.1)
+        return lin
+
+    mod = AwqPackedLinear(DIM, 6 * DIM, bias=True, device="cuda")
+    mod.weight.random_(0, 256)
+    mod.wscales.fill_(2e-4)
+    mod.wzeros.fill_(-15e-4)
+    with torch.no_grad():
+        mod.bias.normal_(0, 0.1)
+    block = torch.nn.ModuleDict({
+        "mod": mod, "norm1": gw.ModulatedLayerNorm(DIM, affine=False, device="cuda"),
+        "norm2": gw.ModulatedLayerNorm(DIM, affine=False, device="cuda"),
+        "qkv": gw.svdq_int4_from_linear(linear(DIM, 3 * DIM)),
+        "out": gw.fp8_rowwise_from_linear(linear(DIM, DIM)),
+        "ff": gw.gated_from_linears(linear(DIM, HIDDEN), linear(DIM, HIDDEN), activation="gelu_tanh",
+                                    down=gw.svdq_int4_from_linear(linear(HIDDEN, DIM))),
+        "rope": gw.RotaryEmbedding(HEAD, interleaved=True, axes=(16, 56, 56), device="cuda"),
+    })
+    return block.requires_grad_(False)
+
+
+def forward(m, x, cond, pos, seen=None):
+    def note(name, *tensors):
+        if seen is not None:
+            seen[name] = [t.clone() for t in tensors]
+
+    shift1, scale1, gate1, shift2, scale2, gate2 = m["mod"](cond).chunk(6, -1)
+    a = m["norm1"](x, scale1, shift1)
+    note("norm1", x, scale1, shift1, a)
+    qkv = m["qkv"](a).view(BATCH, TOKENS, 3 * HEADS, HEAD)
+    q, k = qkv[:, :, :HEADS], qkv[:, :, HEADS:2 * HEADS]
+    qr, kr = m["rope"](q, k, pos)
+    note("rope", q, k, qr, kr)
+    s = torch.einsum("bihd,bjhd->bhij", qr, kr).float() * HEAD ** -0.5
+    att = torch.einsum("bhij,bjhd->bihd", s.softmax(-1).to(x.dtype), qkv[:, :, 2 * HEADS:])
+    x = x + gate1.unsqueeze(1) * m["out"](att.reshape(BATCH, TOKENS, DIM))
+    b = m["norm2"](x, scale2, shift2)
+    note("norm2", x, scale2, shift2, b)
+    ff = m["ff"]
+    if seen is not None:
+        import gen_worker_b200 as gw
+        note("gated", b, gw.gated_linear(b, ff.w_gate, ff.w_up, ff.b_gate, ff.b_up,
+                                         activation=ff.activation))
+    return x + gate2.unsqueeze(1) * ff(b)
+
+
+def inputs(seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(BATCH, TOKENS, DIM, generator=g)
+    x[..., ::100] *= 20                                   # activation outliers
+    cond = torch.randn(BATCH, DIM, generator=g)
+    pos = torch.randint(0, 128, (BATCH, TOKENS, 3), generator=g)
+    return x.bfloat16().cuda(), cond.bfloat16().cuda(), pos.cuda()
+
+
+@pytest.mark.gpu
+def test_block_stages(cuda_ready):
+    """Each new operator against its definition on what the stage before gave it."""
+    m, seen = build(), {}
+    x, cond, pos = inputs(0)
+    with torch.no_grad():
+        y = forward(m, x, cond, pos, seen)
+    assert torch.isfinite(y).all()
+    for name in ("norm1", "norm2"):
+        xin, s, t, out = (v.cpu() for v in seen[name])
+        s, t = s.unsqueeze(1), t.unsqueeze(1)
+        check(out, norm64(xin, s=s, t=t), norm_magnitudes(xin, xin, None, None, s, t, 1e-6)["y"], 80, name)
+    q, k, qr, kr = seen["rope"]
+    rope = m["rope"]
+    for a, b in ((q, qr), (k, kr)):
+        want, mag = rotary64(a.cpu(), pos.cpu(), rope.inv_freq.cpu(), rope.axis.cpu(), True, 1.0)
+        check(b, want, mag, ROTARY_COUNT, "rope")
+    b, h = (v.cpu().flatten(0, 1) for v in seen["gated"])
+    w = [t.detach().cpu() for t in (m["ff"].w_gate, m["ff"].w_up, m["ff"].b_gate, m["ff"].b_up)]
+    h64 = gated64(b, *w, "gelu_tanh")
+    check(h, h64[0], gated_magnitudes(b, *w, None, h64)["h"], 1 / U, "gated")
+
+
+@pytest.mark.gpu
+def test_block_captured(cuda_ready):
+    """The whole block in one graph, replayed on new contents, gives the bits
+    of the eager calls."""
+    from gen_worker_b200 import native
+
+    m = build()
+    with torch.no_grad():
+        want = [forward(m, *inputs(k)) for k in range(3)]
+        x, cond, pos = inputs(0)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            forward(m, x, cond, pos)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = forward(m, x, cond, pos)
+        for k in (2, 1, 0):
+            for dst, src in zip((x, cond, pos), inputs(k)):
+                dst.copy_(src)
+            graph.replay()
+            assert torch.equal(y, want[k])
+    assert native.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("recompute", [False, True])
+def test_training_step(cuda_ready, recompute):
+    """Gradients of norm -> gated -> down -> rotary through a whole step, against
+    64-bit autograd of the same bf16 values. Between x and a gradient lie at most
+    12 tensors rounded to bf16, each off by at most 2^-8 of its own norm (half a
+    step, relative), and none of the maps between them (rotations, a norm of unit
+    rows, products with weights of unit gain) stretches a relative error more
+    than twofold: 12 * 2 * 2^-8 bounds the relative L2 error."""
+    import gen_worker_b200 as gw
+
+    torch.manual_seed(0)
+    dim, hidden = 256, 344
+    ff = gw.GatedFeedForward(dim, hidden, bias=True, recompute=recompute, device="cuda",
+                             down=torch.nn.Linear(hidden, dim, device="cuda", dtype=torch.bfloat16))
+    norm = gw.ModulatedLayerNorm(dim, device="cuda")
+    rope = gw.RotaryEmbedding(64, device="cuda")
+    x, s, t = (torch.randn(*n, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+               for n in ((2, 150, dim), (2, dim), (2, dim)))
+    goal = torch.randn(2, 150, 4, 64, device="cuda", dtype=torch.bfloat16)
+    pos = torch.arange(150, device="cuda")
+    leaves = {"x": x, "scale": s, "shift": t, **dict(norm.named_parameters()),
+              **{n: p for n, p in ff.named_parameters()}}
+    y, _ = rope((x + ff(norm(x, s, t))).view(2, 150, 4, 64), None, pos)
+    (y * goal).sum().backward()
+
+    r = {n: p.detach().cpu().double().requires_grad_(True) for n, p in leaves.items()}
+    b = norm64(r["x"], r["weight"], r["bias"], r["scale"].unsqueeze(1), r["shift"].unsqueeze(1))
+    h = gated64(b.flatten(0, 1), r["w_gate"], r["w_up"], r["b_gate"], r["b_up"], "silu")[0]
+    z = r["x"] + (h @ r["down.weight"].t() + r["down.bias"]).view(2, 150, dim)
+    z = z.view(2, 150, 4, 64)
+    ang = pos.cpu().double()[:, None] * rope.inv_freq.cpu()
+    c, sn = ang.cos()[:, None], ang.sin()[:, None]
+    p, q = z[..., :32], z[..., 32:]
+    out = torch.cat([p * c - q * sn, q * c + p * sn], -1)
+    (out * goal.cpu().double()).sum().backward()
+    for n, leaf in leaves.items():
+        got, want = leaf.grad.double().cpu(), r[n].grad
+        rel = float((got - want).norm() / want.norm())
+        assert rel <= 12 * 2 * 2.0 ** -8, (n, rel)
+
+
+def test_package_lists_the_operators():
+    """The entry points are exported, and the library has the C functions."""
+    import gen_worker_b200 as gw
+    from gen_worker_b200 import native
+
+    for name in ("layer_norm", "ModulatedLayerNorm", "rotary", "rotary_", "RotaryEmbedding",
+                 "gated_linear", "GatedFeedForward"):
+        assert name in gw.__all__ and callable(getattr(gw, name))
+    lib = native.lib()
+    for name in native.EXPORTED:
+        assert hasattr(lib, name)
+
+
+def test_fake_tensors_trace_through():
+    """Shapes and types for torch.compile, without a GPU."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import gen_worker_b200 as gw
+
+    with FakeTensorMode():
+        x = torch.empty(2, 5, 64, device="cuda", dtype=torch.bfloat16)
+        w = torch.empty(72, 64, device="cuda", dtype=torch.bfloat16)
+        assert gw.layer_norm(x).shape == x.shape
+        assert gw.gated_linear(x, w, w).shape == (2, 5, 72)
+        q, k = gw.rotary(x.view(2, 5, 2, 32), None, torch.empty(5, device="cuda", dtype=torch.int64),
+                         torch.empty(8, device="cuda", dtype=torch.float64))
+        assert q.shape == (2, 5, 2, 32) and k is None
