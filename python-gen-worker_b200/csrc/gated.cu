@@ -436,7 +436,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
           if (Kept<T>::scaled && row < a.M) {
             const int groups = (a.F + 63) / 64;
             a.kept_scale[(size_t)row * groups + n0 / 64] = sa;
-            a.kept_scale[(size_t)(a.M + row) * groups + n0 / 64] = sb;
+            a.kept_scale[((size_t)a.M + row) * groups + n0 / 64] = sb;
           }
           K* ka = static_cast<K*>(a.kept) + (size_t)row0 * a.F + n0;
           put(ka, 0, sa);
@@ -684,7 +684,7 @@ gradients_kernel(const T* __restrict__ dh, int64_t dhs, const void* __restrict__
           load8(ka + plane, u);
           // the scales are powers of two: their reciprocals are exact
           ra = 1.0f / __ldg(scale + (size_t)r * groups + c0 / 64);
-          rb = 1.0f / __ldg(scale + (size_t)(M + r) * groups + c0 / 64);
+          rb = 1.0f / __ldg(scale + ((size_t)M + r) * groups + c0 / 64);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; j += 4) {

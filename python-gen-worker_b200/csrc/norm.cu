@@ -106,8 +106,8 @@ __device__ __forceinline__ Span span_of(const T* first, int64_t n) {
 
 // One thread: the copy of n elements at `first` to dst, to complete on `bar`
 // (whose expected bytes the caller has not announced yet); returns them.
-// `last`: nothing may be read behind the elements, so a part granule at the
-// end is stored by hand, ordered before the copy's completion by this
+// `last` (the last row, or rows that lie on top of each other): nothing may be
+// read behind the elements, so a part granule at the end is stored by hand, ordered before the copy's completion by this
 // thread's own arrival.
 template <typename T>
 __device__ __forceinline__ uint32_t span_bytes(const T* first, int64_t n, bool last, uint8_t* dst) {
@@ -209,7 +209,7 @@ forward_kernel(const FwdArgs a, const FwdPlan p) {
     const int64_t n = (rows - 1) * a.D + a.D;            // one row, or rows that adjoin
     uint8_t* dst = ring + (size_t)(s % p.stages) * p.slot_bytes;
     const T* src = x + r * a.xs;
-    const uint32_t bytes = span_bytes(src, n, r + rows == a.M, dst);
+    const uint32_t bytes = span_bytes(src, n, r + rows == a.M || a.xs < a.D, dst);
     mbar_arrive_expect_tx(&full[s % p.stages], bytes);
     if (bytes) bulk_load(dst, span_of(src, n).from, bytes, &full[s % p.stages]);
   };
@@ -614,7 +614,8 @@ backward_staged_kernel(const BwdArgs a, const BwdPlan p) {
     const int r = s * R + (lane >> 1);
     const T* src = lane & 1 ? dy + r * a.dys : x + r * a.xs;
     uint8_t* dst = ring + slot * slot_bytes + lane * p.x_slot;
-    const uint32_t bytes = r < count ? span_bytes(src, a.D, base + r == p.last, dst) : 0u;
+    const bool last = base + r == p.last || (lane & 1 ? a.dys : a.xs) < a.D;
+    const uint32_t bytes = r < count ? span_bytes(src, a.D, last, dst) : 0u;
     mbar_arrive_expect_tx(&full[slot], bytes);
     if (bytes) bulk_load(dst, span_of(src, a.D).from, bytes, &full[slot]);
   };

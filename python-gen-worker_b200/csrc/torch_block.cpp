@@ -10,9 +10,11 @@
 // build a graph of its own is refused.
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/library.h>
 
@@ -66,6 +68,29 @@ void refuse_second_order(const char* what, const Ts&... ts) {
   if (!at::GradMode::is_enabled()) return;
   const bool any = (wants(ts) || ...);
   TORCH_CHECK(!any, what, " has no second derivative (create_graph=True)");
+}
+
+// While a graph that used a leaf lives, torch keeps that leaf's gradient on the
+// stream of that graph. A backward pass captured on another stream would have
+// to wait for it across the capture, which breaks the capture in the middle of
+// the engine's work. Refused here, where the forward call is captured.
+void refuse_foreign_leaf(const char* what, const Tensor& t) {
+  if (!wants(t) || !t.is_leaf() || !t.is_cuda()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto stream = node->stream();
+  const c10::Stream now = c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap();
+  TORCH_CHECK(!stream.has_value() || *stream == now, what,
+              " is captured while a graph of the same leaf lives on another stream: capture with"
+              " leaves of its own (t.detach().requires_grad_()), or let that graph go first");
+}
+void refuse_foreign_leaf(const char* what, const OptTensor& t) {
+  if (has(t)) refuse_foreign_leaf(what, *t);
+}
+template <typename... Ts>
+void refuse_foreign_leaves(const char* what, const Ts&... ts) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  (refuse_foreign_leaf(what, ts), ...);
 }
 
 // Whether [..., D] lies as rows at one stride; that stride.
@@ -281,8 +306,10 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 Tensor layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b,
                            const OptTensor& scale, const OptTensor& shift, double eps) {
   if (at::GradMode::is_enabled() &&
-      (wants(x) || wants(w) || wants(b) || wants(scale) || wants(shift)))
+      (wants(x) || wants(w) || wants(b) || wants(scale) || wants(shift))) {
+    refuse_foreign_leaves("layer_norm", x, w, b, scale, shift);
     return LayerNormFn::apply(x, w, b, scale, shift, eps);
+  }
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = op_of<decltype(layer_norm_cuda)>("gwb200::layer_norm");
   return op.call(x, w, b, scale, shift, eps);
@@ -480,6 +507,7 @@ std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptTensor& k,
                                            const OptTensor& axis, bool interleaved, double scale,
                                            bool inverse) {
   if (at::GradMode::is_enabled() && (wants(q) || wants(k))) {
+    refuse_foreign_leaves("rotary", q, k);
     auto r = RotaryFn::apply(q, k, positions, inv_freq, axis, interleaved, scale, inverse);
     return {r[0], r[1]};
   }
@@ -664,8 +692,10 @@ Tensor gated_linear_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu
                              const OptTensor& bg, const OptTensor& bu, int64_t act,
                              bool recompute) {
   if (at::GradMode::is_enabled() &&
-      (wants(x) || wants(wg) || wants(wu) || wants(bg) || wants(bu)))
+      (wants(x) || wants(wg) || wants(wu) || wants(bg) || wants(bu))) {
+    refuse_foreign_leaves("gated_linear", x, wg, wu, bg, bu);
     return GatedLinearFn::apply(x, wg, wu, bg, bu, act, recompute);
+  }
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = op_of<decltype(gated_linear_cuda)>("gwb200::gated_linear");
   return op.call(x, wg, wu, bg, bu, act, recompute);

@@ -168,6 +168,49 @@ def test_training_step(cuda_ready, recompute):
         assert rel <= 12 * 2 * 2.0 ** -8, (n, rel)
 
 
+@pytest.mark.gpu
+def test_captured_backward_beside_an_eager_graph(cuda_ready):
+    """Capturing a pass with gradients while an eager graph of the same leaves
+    lives is refused where it begins; leaves of its own, or no such graph, and
+    it gives the eager bits."""
+    import gen_worker_b200 as gw
+
+    x = torch.randn(40, 64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    w = torch.randn(72, 64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    rope = gw.RotaryEmbedding(16, device="cuda")
+    pos = torch.arange(40, device="cuda")
+    calls = [lambda x, w: gw.layer_norm(x), lambda x, w: gw.gated_linear(x, w, w),
+             lambda x, w: rope(x.view(40, 4, 16), None, pos)[0]]
+
+    def capture(call, x, w):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(x, w)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call(x, w)
+            out = torch.autograd.grad(y, x, torch.ones_like(y))
+        return graph, out
+
+    for i, call in enumerate(calls):
+        y = call(x, w)                                   # the eager graph lives
+        if i < 2:                                        # rotary's q is a view: no leaf of its own
+            with pytest.raises(RuntimeError, match="leaves of its own"):
+                capture(call, x, w)
+        mine = [t.detach().requires_grad_(True) for t in (x, w)]
+        graph, inside = capture(call, *mine)
+        graph.replay()
+        outside, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert torch.equal(inside[0], outside)
+        del y, inside, graph
+        graph, inside = capture(call, x, w)              # and with it gone
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(inside[0], outside)
+
+
 def test_package_lists_the_operators():
     """The entry points are exported, and the library has the C functions."""
     import gen_worker_b200 as gw

@@ -130,6 +130,25 @@ def test_row_strides_and_chunks(cuda_ready, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [96, 101, 700, 1153])
+def test_rows_on_top_of_each_other(cuda_ready, d):
+    """One row seen as many (stride 0), as x and as the gradient."""
+    from gen_worker_b200 import layer_norm
+
+    row = torch.randn(d, generator=torch.Generator().manual_seed(d)).to(torch.bfloat16)
+    x = row.cuda().expand(37, d).detach().requires_grad_(True)
+    y = layer_norm(x)
+    g, = torch.autograd.grad(y, x, row.cuda().expand(37, d))
+    xc, dy = row.expand(37, d), row.expand(37, d)
+    r = xc.double().requires_grad_(True)
+    want = norm64(r)
+    wg, = torch.autograd.grad(want, r, dy.double())
+    m = norm_magnitudes(xc, dy, None, None, None, None, 1e-6)
+    check(y, want, m["y"], ROW, "y")
+    check(g, wg, m["x"], ROW, "x")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_constant_rows_far_means_and_bad_values(cuda_ready, dtype):
     from gen_worker_b200 import layer_norm
