@@ -175,9 +175,9 @@ struct FwdPlan {
 
 // A warp takes whole rows (32 / L at a time, L lanes each), E elements a
 // lane, from its own ring of bulk copies: no barrier but the one that shares
-// g and h, and few instructions a row besides the arithmetic, which a form
-// with a CTA per row spent on its reductions (21 us against 12 at 4608 x 2304
-// bf16). VECTOR: rows and parameters lie on 16 bytes, a lane has vectors
+// g and h, and few instructions a row besides the arithmetic (18432 x 3072
+// bf16 with scale and shift: 45 us, 5.0 TB/s; without parameters 33, 6.8 TB/s:
+// the rest is g and h coming out of shared memory for every row). VECTOR: rows and parameters lie on 16 bytes, a lane has vectors
 // lane, lane + L, ...; else elements lane, lane + L, ..., so that any
 // alignment reads shared memory without conflicts.
 template <typename T, int E, int LO, int L, bool VECTOR>
@@ -421,6 +421,106 @@ __global__ void __launch_bounds__(512) forward_block_kernel(const FwdArgs a) {
   }
 }
 
+// The same for rows and parameters on 16 bytes, in packed f32: C vectors a
+// thread, its parameters read as vectors where they are used. Two barriers a
+// row, but thousands of CTAs to hide them behind: it beats the warp a row, with
+// its g and h to prepare and rows to take in turn, up to a few rows a warp (1024
+// and 4608 rows of 3072 bf16: 9.8 and 16.5 us a call against 13.4 and 18.5).
+template <typename T>
+__device__ __forceinline__ void load_pairs(const Param& a, int64_t b, int c,
+                                           F2 (&o)[Pairs<T>::N]) {
+  if (a.f32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.p) + b * a.stride + c);
+#pragma unroll
+    for (int j = 0; j < Pairs<T>::N; j += 2) {
+      const float4 f = __ldg(p + j / 2);
+      o[j] = f2(f.x, f.y);
+      o[j + 1] = f2(f.z, f.w);
+    }
+  } else {
+    unpack<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.p) + b * a.stride + c)), o);
+  }
+}
+
+template <typename T, int C>
+__global__ void __launch_bounds__(512) forward_pairs_kernel(const FwdArgs a) {
+  constexpr int VEC = 16 / (int)sizeof(T), P = Pairs<T>::N;
+  __shared__ float red[2][16];
+  const int lanes = blockDim.x, t = threadIdx.x, nw = lanes >> 5, nvec = a.D / VEC;
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.xs;
+  const float inv_d = 1.0f / (float)a.D;
+  const auto total = [&](F2 v, int k) {
+    const float w = warp_sum(sum2(v));
+    if (nw == 1) return w;
+    if ((t & 31) == 0) red[k][t >> 5] = w;
+    __syncthreads();
+    float s = 0.0f;
+    for (int i = 0; i < nw; ++i) s += red[k][i];
+    return s;
+  };
+  uint4 raw[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    raw[c] = t + c * lanes < nvec ? *reinterpret_cast<const uint4*>(x + (t + c * lanes) * VEC)
+                                  : make_uint4(0, 0, 0, 0);
+  F2 v[C][P], acc = f2(0.0f, 0.0f);
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    unpack<T>(raw[c], v[c]);
+#pragma unroll
+    for (int j = 0; j < P; ++j) acc = add2(acc, v[c][j]);
+  }
+  const float mean = total(acc, 0) * inv_d;
+  const F2 neg = f2(-mean, -mean);
+  acc = f2(0.0f, 0.0f);
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (t + c * lanes < nvec)
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        v[c][j] = add2(v[c][j], neg);
+        acc = fma2(v[c][j], v[c][j], acc);
+      }
+  const float rstd = rsqrtf(total(acc, 1) * inv_d + a.eps);
+  if (t == 0 && a.mean != nullptr) {
+    a.mean[row] = mean;
+    a.rstd[row] = rstd;
+  }
+  const int64_t smp = a.s.p || a.t.p ? row / a.rows_per_mod : 0;
+  const F2 r2 = f2(rstd, rstd), one = f2(1.0f, 1.0f);
+  T* y = static_cast<T*>(a.y) + row * a.D;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int i = t + c * lanes;
+    if (i >= nvec) continue;
+    F2 p[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) v[c][j] = mul2(v[c][j], r2);
+    if (a.w.p) {
+      load_pairs<T>(a.w, 0, i * VEC, p);
+#pragma unroll
+      for (int j = 0; j < P; ++j) v[c][j] = mul2(v[c][j], p[j]);
+    }
+    if (a.b.p) {
+      load_pairs<T>(a.b, 0, i * VEC, p);
+#pragma unroll
+      for (int j = 0; j < P; ++j) v[c][j] = add2(v[c][j], p[j]);
+    }
+    if (a.s.p) {
+      load_pairs<T>(a.s, smp, i * VEC, p);
+#pragma unroll
+      for (int j = 0; j < P; ++j) v[c][j] = mul2(v[c][j], add2(one, p[j]));
+    }
+    if (a.t.p) {
+      load_pairs<T>(a.t, smp, i * VEC, p);
+#pragma unroll
+      for (int j = 0; j < P; ++j) v[c][j] = add2(v[c][j], p[j]);
+    }
+    *reinterpret_cast<uint4*>(y + i * VEC) = repack<T>(v[c]);
+  }
+}
+
 // Rows too wide for the registers of one CTA: three passes, the second and
 // third from L2.
 template <typename T>
@@ -588,8 +688,8 @@ struct BwdPlan { int stages; uint32_t x_slot; int64_t last; };
 // and of both column sums in registers for the whole chunk; the second pass
 // over a slot (dx) reads it from shared memory again, because holding it would
 // halve the warps a multiprocessor runs, and their number is what hides the
-// latencies here (a form with 16 columns a thread and half the warps took 115
-// us against 94 at 18432 x 2304 bf16). A slot is filled again after the next
+// latencies here (16 columns a thread and half the warps took 90 us against 79
+// at 18432 x 3072 bf16, 4.3 TB/s; issue slots are 59 % busy). A slot is filled again after the next
 // step's barrier. Every wait is bounded, and all threads leave together.
 template <typename T, int E, bool VECTOR>
 __global__ void __launch_bounds__(E <= 8 ? 416 : E <= 16 ? 512 : 384, E <= 8 ? 2 : 1)
@@ -987,10 +1087,34 @@ int forward_v(const FwdArgs& a, cudaStream_t st) {
   return launch_status();
 }
 
+// A CTA a row rather than a warp a row: up to 56 rows a multiprocessor, and for
+// wide f32 rows, whose copies leave the other form too few warps (18432 x 3072
+// f32: 86 us against 99; bf16: 60 against 50).
+inline bool pairs_fit(const FwdArgs& a, int V) {
+  if (a.D / V <= 32 || a.D > 4096) return false;
+  return (V == 4 && a.D > 2048) || a.M <= (int64_t)sm_count() * 56;
+}
+template <typename T>
+int forward_pairs(const FwdArgs& a, cudaStream_t st) {
+  // three vectors a thread, up to 512 threads
+  const int nvec = a.D / (16 / (int)sizeof(T));
+  int th = 32;
+  while (th < 512 && nvec > th * 3) th *= 2;
+  const int c = (nvec + th - 1) / th;
+  const unsigned m = (unsigned)a.M;
+  if (c <= 1) forward_pairs_kernel<T, 1><<<m, th, 0, st>>>(a);
+  else if (c <= 2) forward_pairs_kernel<T, 2><<<m, th, 0, st>>>(a);
+  else if (c <= 3) forward_pairs_kernel<T, 3><<<m, th, 0, st>>>(a);
+  else forward_pairs_kernel<T, 4><<<m, th, 0, st>>>(a);
+  return launch_status();
+}
+
 template <typename T>
 int forward_t(const FwdArgs& a, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   const bool vector = a.D % V == 0 && a.xs % V == 0 && aligned16(a.x) && aligned16(a.y);
+  if (vector && pairs_fit(a, V) && vector_ok<T>(a.D, {}, {}, {a.w, a.b, a.s, a.t}))
+    return forward_pairs<T>(a, st);
   return vector ? forward_v<T, true>(a, st) : forward_v<T, false>(a, st);
 }
 
