@@ -211,6 +211,85 @@ def test_captured_backward_beside_an_eager_graph(cuda_ready):
         assert torch.equal(inside[0], outside)
 
 
+@pytest.mark.gpu
+def test_two_streams_at_once(cuda_ready):
+    """The same calls from two streams at the same time share nothing."""
+    import gen_worker_b200 as gw
+
+    g = torch.Generator().manual_seed(4)
+    sets = [[torch.randn(*n, generator=g).bfloat16().cuda() for n in ((600, 512), (776, 512), (776, 512),
+                                                                     (600, 776))] for _ in range(2)]
+    pos = torch.arange(600, device="cuda")
+    rope = gw.RotaryEmbedding(64, device="cuda")
+
+    def step(x, wg, wu, dh):
+        x = x.detach().requires_grad_(True)
+        a = gw.layer_norm(x)
+        b, _ = rope(a.view(600, 8, 64), None, pos)
+        h = gw.gated_linear(b.reshape(600, 512), wg, wu)
+        small = gw.gated_linear(b.reshape(600, 512)[:9], wg, wu)
+        return [h.detach(), small.detach(), *torch.autograd.grad(h, x, dh)]
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(step(*sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(a, b) for run in got[k] for a, b in zip(run, want[k]))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda_ready):
+    """Tensors of over 2^31 elements: the last rows come out as the definition
+    has them, and sums over all rows count every one."""
+    import gen_worker_b200 as gw
+
+    def near(got, want, count):
+        """Within one rounding and `count` f32 roundings of unit values."""
+        tol = 2.0 ** -8 * want.abs() + count * U * 8
+        assert ((got.double() - want).abs() <= tol).all()
+
+    # norm: 2.2e9 elements; ones in dy make the column sums row counts
+    rows, dim = 270_000, 8192
+    x = torch.empty(rows, dim, device="cuda", dtype=torch.bfloat16).normal_().requires_grad_(True)
+    w = torch.ones(dim, device="cuda").requires_grad_(True)
+    b = torch.zeros(dim, device="cuda").requires_grad_(True)
+    y = gw.layer_norm(x, w, b)
+    tail = x.detach()[-3:].double()
+    near(y.detach()[-3:], (tail - tail.mean(1, keepdim=True)) / tail.var(1, correction=0, keepdim=True)
+         .add(1e-6).sqrt(), 80)
+    dy = torch.ones_like(x)
+    gx, gb = torch.autograd.grad(y, [x, b], dy)
+    assert torch.equal(gb, torch.full_like(gb, float(rows)))
+    near(gx[-3:], torch.zeros(3, dim, device="cuda", dtype=torch.float64), 400)
+    del x, y, dy, gx, tail
+    # rotary: one head's last tokens
+    q = torch.empty(1, 4_200_000, 4, 128, device="cuda", dtype=torch.bfloat16).normal_()
+    pos = torch.arange(4_200_000, device="cuda") % 5000
+    rope = gw.RotaryEmbedding(128, device="cuda")
+    qo, _ = rope(q, None, pos)
+    again, _ = rope(q[:, -50:].clone(), None, pos[-50:])
+    assert torch.equal(qo[:, -50:], again)
+    del q, qo
+    # gated: h of 2.2e9 elements, with its backward pass
+    rows, dim, hidden = 180_000, 64, 12288
+    x = torch.randn(rows, dim, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    wg, wu = (torch.randn(hidden, dim, device="cuda", dtype=torch.bfloat16) * 0.1 for _ in range(2))
+    h = gw.gated_linear(x, wg, wu)
+    few = x.detach()[-200:].clone().requires_grad_(True)
+    part = gw.gated_linear(few, wg, wu)
+    assert torch.equal(h.detach()[-200:], part)
+    dh = torch.ones_like(h)
+    gx, = torch.autograd.grad(h, x, dh)
+    gp, = torch.autograd.grad(part, few, dh[:200])
+    assert float((gx[-200:].double() - gp.double()).norm() / gp.double().norm()) <= 2.0 ** -8
+
+
 def test_package_lists_the_operators():
     """The entry points are exported, and the library has the C functions."""
     import gen_worker_b200 as gw
