@@ -577,7 +577,7 @@ __device__ __forceinline__ void gain(const Param& w, const Param& s, int64_t smp
 // sample's rows, its eight warps rows in turn, one a warp; a thread keeps its
 // C vectors of columns, joined over the warps at the end.
 template <typename T, int VEC, int C>
-__global__ void __launch_bounds__(256) backward_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(256, C == 1 ? 4 : 2) backward_kernel(const BwdArgs a) {
   extern __shared__ float part_sm[];             // [8][2][D]
   const int warp = threadIdx.x >> 5, t = threadIdx.x & 31;
   const int nvec = a.D / VEC;
@@ -614,30 +614,62 @@ __global__ void __launch_bounds__(256) backward_kernel(const BwdArgs a) {
     for (int c = 0; c < C; ++c) { xv[c] = xn[c]; dv[c] = dn[c]; }
     if (r + 8 < r1) fetch(r + 8);
     float sa = 0.0f, sb = 0.0f;
+    if constexpr (VEC > 1) {
+      constexpr int P = VEC / 2;
+      const F2 neg = f2(-mean, -mean), r2 = f2(rstd, rstd);
+      F2 ta = f2(0.0f, 0.0f), tb = ta;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (t + c * 32 < nvec)
+      for (int c = 0; c < C; ++c)
+        if (t + c * 32 < nvec) {
+          F2 x2[P], d2[P];
+          unpack<T>(xv[c].bits(), x2);
+          unpack<T>(dv[c].bits(), d2);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float z = (xv[c].get(j) - mean) * rstd, d = dv[c].get(j), e = d * z;
-          s1[c][j] += d;
-          s2[c][j] += e;
-          sa += d * g[c][j];
-          sb += e * g[c][j];
+          for (int j = 0; j < P; ++j) {
+            const F2 g2 = f2(g[c][2 * j], g[c][2 * j + 1]), q = mul2(d2[j], add2(x2[j], neg));
+            const float2 u = split(add2(f2(s1[c][2 * j], s1[c][2 * j + 1]), d2[j]));
+            const float2 w = split(fma2(q, r2, f2(s2[c][2 * j], s2[c][2 * j + 1])));
+            s1[c][2 * j] = u.x; s1[c][2 * j + 1] = u.y;
+            s2[c][2 * j] = w.x; s2[c][2 * j + 1] = w.y;
+            ta = fma2(d2[j], g2, ta);
+            tb = fma2(q, g2, tb);
+          }
         }
+      sa = sum2(ta);
+      sb = sum2(tb) * rstd;
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (t + c * 32 < nvec) {
+          const float z = (xv[c].get(0) - mean) * rstd, d = dv[c].get(0), e = d * z;
+          s1[c][0] += d;
+          s2[c][0] += e;
+          sa += d * g[c][0];
+          sb += e * g[c][0];
+        }
+    }
     if (a.dx == nullptr) continue;
     const float ma = warp_sum(sa) * inv_d, mb = warp_sum(sb) * inv_d;
+    // dx = rstd (d g - A - z B) = (d g) rstd + (x c1 + c0)
+    const float c1 = -rstd * rstd * mb, c0 = -mean * c1 - rstd * ma;
     T* dx = static_cast<T*>(a.dx) + (base + r) * a.D;
 #pragma unroll
     for (int c = 0; c < C; ++c)
       if (t + c * 32 < nvec) {
-        Pack<T, VEC> o;
+        if constexpr (VEC > 1) {
+          constexpr int P = VEC / 2;
+          F2 x2[P], d2[P];
+          unpack<T>(xv[c].bits(), x2);
+          unpack<T>(dv[c].bits(), d2);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float z = (xv[c].get(j) - mean) * rstd;
-          o.set(j, rstd * (dv[c].get(j) * g[c][j] - ma - z * mb));
+          for (int j = 0; j < P; ++j)
+            d2[j] = fma2(mul2(d2[j], f2(g[c][2 * j], g[c][2 * j + 1])), f2(rstd, rstd),
+                         fma2(x2[j], f2(c1, c1), f2(c0, c0)));
+          xv[c].put(repack<T>(d2));
+          xv[c].store(dx + (t + c * 32) * VEC);
+        } else {
+          dx[t + c * 32] = from_f32<T>(dv[c].get(0) * g[c][0] * rstd + (xv[c].get(0) * c1 + c0));
         }
-        o.store(dx + (t + c * 32) * VEC);
       }
   }
   if (a.partial == nullptr) return;
