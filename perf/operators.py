@@ -284,18 +284,12 @@ def _plain_gated(st):
 
 
 # ---------------------------------------------------------------- the framework's calls
-_imported = []
-
-
 def _package():
-    """The package, imported once as a program's import line does."""
-    if not _imported:
-        root = str(Path(__file__).resolve().parent.parent / "python-gen-worker_b200")
-        if root not in sys.path:
-            sys.path.insert(0, root)
-        import gen_worker_b200
-        _imported.append(gen_worker_b200)
-    return _imported[0]
+    root = str(Path(__file__).resolve().parent.parent / "python-gen-worker_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import gen_worker_b200
+    return gen_worker_b200
 
 
 def _own_run(st):
