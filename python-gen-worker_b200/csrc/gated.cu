@@ -637,6 +637,9 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
             for (int j = 0; j < 16; ++j)
               if (16 * c + j < a.M)
                 static_cast<T*>(a.o0)[(size_t)(16 * c + j) * a.F + f] = from_f32<T>(h[j]);
+          // lanes past w or F stored nothing: together again for the next
+          // accumulator load and the barrier, which take whole warps
+          __syncwarp();
         }
       }
       tc_fence_before();

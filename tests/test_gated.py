@@ -111,6 +111,22 @@ def test_split_products(cuda_ready, m, d, f, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("f", [12288, 148 * 40, 13096])
+@pytest.mark.parametrize("m", [33, 100, 128])
+def test_few_rows_whose_tiles_end_inside_a_warp(cuda_ready, m, f, dtype):
+    """Two chunks of rows or more for each half of the epilogue, and tiles of 88
+    and 40 features, so a warp's lanes part at the stores of every chunk, or of
+    96, the last of which ends inside a warp."""
+    p = make(m, 72, f, dtype, bias=m == 100)
+    from gen_worker_b200 import gated_linear
+
+    h = gated_linear(*(p[n].cuda() for n in ("x", "w_gate", "w_up")),
+                     *(p[n].cuda() for n in ("b_gate", "b_up") if n in p))
+    verify(p, "silu", h, None)
+
+
+@pytest.mark.gpu
 def test_many_tiles(cuda_ready):
     """More tiles than multiprocessors, so the persistent walk wraps."""
     p = make(1100, 520, 2600, torch.bfloat16, bias=True)
