@@ -333,8 +333,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
     for (int tile = pair; tile < a.ntiles; tile += pairs, ++lt) {
       const Tile t = tile_of<MODE>(a, PROJ ? tile : tile / a.parts);
       const int b = lt & 1;
-      if (!mbar_wait(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
-      __syncwarp();
+      if (!mbar_wait_warp(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
       uint32_t v[128];
       const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + b * BN;
@@ -603,7 +602,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
     bool ok = true;
     for (int tile = blockIdx.x; tile < a.ntiles; tile += gridDim.x, ++lt) {
       const int b = lt & 1;
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE));
+      ok = ok && mbar_wait_warp(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE);
       tc_fence_after();
       const int f = tile * w + fl;
       const bool mine = fl < w && f < a.F;
@@ -622,6 +621,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
       if (FT == 128 || q < 2) {
         const float bg = a.bg && mine ? to_f32<T>(static_cast<const T*>(a.bg)[f]) : 0.0f;
         const float bu = a.bu && mine ? to_f32<T>(static_cast<const T*>(a.bu)[f]) : 0.0f;
+        __syncwarp();
         for (int c = half; c < chunks; c += 2) {
           tmem_ld16(base + 16 * c, v);
           if (FT == 128) tmem_ld16(base + 128 + 16 * c, vu);

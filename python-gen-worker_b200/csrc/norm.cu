@@ -244,7 +244,7 @@ forward_kernel(const FwdArgs a, const FwdPlan p) {
   T* y = static_cast<T*>(a.y);
   int slot = 0, phase = 0;
   for (int s = 0; s < steps; ++s) {
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], phase, GWB_ERR_TIMEOUT_ACT))) {
+    if (!mbar_wait_warp(&full[slot], phase, GWB_ERR_TIMEOUT_ACT)) {
       if (lane == 0) drain(full, p.stages, s, min(steps, s + p.stages));
       return;
     }

@@ -92,6 +92,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int er
   return false;
 }
 
+// The same for a whole warp: one outcome for all lanes, and the warp together
+// after it (accumulator loads take whole warps, and lanes may otherwise differ
+// on a wait that runs out).
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
