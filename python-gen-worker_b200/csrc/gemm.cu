@@ -174,7 +174,7 @@ gemm_w8a8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++lt) {
       const int m0 = (tile / tiles_n) * kBM, n0 = (tile % tiles_n) * BN;
       const int b = lt & 1;
-      if (!mbar_wait(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
+      if (!mbar_wait_warp(&acc_full[b], (lt >> 1) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
       // the whole 32-row x 128-column slice goes to registers, then the
       // accumulator is handed back before any arithmetic
@@ -604,7 +604,7 @@ gemm_w4a4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     for (int j = 0; j < EC / 2; ++j) acc[j] = make_float2(0.f, 0.f);
     for (int gt = 0; gt < total; ++gt, ++gi) {
       const int b = gi % NBUF;
-      if (!mbar_wait(&acc_full[b], (gi / NBUF) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+      if (!mbar_wait_warp(&acc_full[b], (gi / NBUF) & 1, GWB_ERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
       if (warp == EPI0 && lane == 0) GWB_TRACE_AT(5, gi);
       tc_fence_after();
       const uint32_t col0 = lane_base + b * BN + cb;
@@ -922,7 +922,7 @@ gemm_nvfp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     int lt = 0;
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x, ++lt) {
       const int m0 = (tile / tiles_n) * kBM, n0 = (tile % tiles_n) * BN;
-      if (!mbar_wait(acc_full, lt & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
+      if (!mbar_wait_warp(acc_full, lt & 1, GWB_ERR_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
       uint32_t v[EC];
       const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + ACC_COL + cb;

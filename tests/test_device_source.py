@@ -9,7 +9,7 @@ import pytest
 CSRC = Path(__file__).resolve().parent.parent / "python-gen-worker_b200" / "csrc"
 
 
-@pytest.mark.parametrize("name", ["gated.cu"])
+@pytest.mark.parametrize("name", ["gated.cu", "gemm.cu"])
 def test_epilogue_waits_take_the_whole_warp(name):
     """Accumulator loads need every lane of the warp. A bounded wait may run out
     in some lanes and not in others, so a role that reads accumulators must
