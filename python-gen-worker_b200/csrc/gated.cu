@@ -107,7 +107,9 @@ __device__ __forceinline__ ActValue activation(float g) {
   ActValue r;
   r.slope = 0.0f;
   if constexpr (KIND == GWB_ACT_GELU) {
-    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    // erfc, not 1 + erf, which cancels for negative g: off by 4 % at -5, all of
+    // it from -5.6 on
+    const float cdf = 0.5f * erfcf(g * -0.70710678118654752f);
     r.act = g * cdf;
     if (SLOPE) r.slope = cdf + g * (0.39894228040143268f * __expf(-0.5f * g * g));
   } else {

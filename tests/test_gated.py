@@ -225,6 +225,50 @@ def test_non_finite_rows_stay_alone(cuda_ready):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [2, 150])
+def test_negative_tail_is_relative(cuda_ready, m, act, dtype):
+    """Gates in [-5.5, -3], where act(g) falls to 1e-7: h and the gradients keep
+    their accuracy relative to act(g) and act'(g). Row 0 of x is a unit vector
+    and the others are zero, so g and u are single exact products and the bias
+    gradients are row 0's dg and du alone.
+
+    f32 roundings (U) of act and act': the argument of exp or erfc is off by up
+    to 4 U of at most 21, which the function turns into 84 U of its value; exp's
+    own error is 2 + 1.16 * 21 ulp, 54 U, erfc's 8 U; products and the sum of
+    two terms of which neither is over 8 times the result, 20 U: 160 U. Each
+    output adds its rounding, and dg and du for bf16 that of a kept f16."""
+    f = 64 * 5
+    g = -torch.linspace(3.0, 5.5, f).to(dtype)
+    up = 1024.0                                   # keeps f16's h out of its subnormals
+    p = {"x": torch.zeros(m, 8, dtype=dtype), "w_gate": torch.zeros(f, 8, dtype=dtype),
+         "w_up": torch.zeros(f, 8, dtype=dtype), "b_gate": torch.zeros(f, dtype=dtype),
+         "b_up": torch.zeros(f, dtype=dtype), "dh": torch.zeros(m, f, dtype=dtype)}
+    p["x"][0, 0], p["dh"][0] = 1.0, 1.0
+    p["w_gate"][:, 0], p["w_up"][:, 0] = g, up
+    g64 = g.double().requires_grad_(True)
+    a64 = gated64(torch.ones(1, 1), g64[:, None], torch.ones(f, 1), None, None, act)[0][0]
+    slope, = torch.autograd.grad(a64.sum(), g64)
+    a64 = a64.detach()
+    step, kept = half_step(dtype), half_step(torch.float16) if dtype == torch.bfloat16 else 0.0
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+    def near(got, want, extra, what):
+        off = (got.detach().double().cpu() - want).abs()
+        bound = want.abs() * (160 * U + extra) * (1 + 2 * step) + step * want.abs() + tiny
+        assert (off <= bound).all(), (what, float((off / want.abs()).max()), float(g[off.argmax()]))
+
+    for recompute in (False, True):
+        h, grads = run(p, act, recompute=recompute)
+        near(h[0], a64 * up, 0.0, "h")
+        assert not h[1:].any()
+        near(grads["b_gate"], slope * up, 0.0 if recompute else kept, "dg")
+        near(grads["b_up"][a64.abs() > 2 * torch.finfo(dtype).smallest_normal],
+             a64[a64.abs() > 2 * torch.finfo(dtype).smallest_normal], 0.0 if recompute else kept, "du")
+
+
+@pytest.mark.gpu
 def test_no_rows(cuda_ready):
     p = make(0, 64, 128, torch.bfloat16, bias=True)
     h, g = run(p)
