@@ -86,11 +86,18 @@ struct Args {
 template <typename T> struct Kept { using type = __half; static constexpr bool scaled = true; };
 template <> struct Kept<__half> { using type = float; static constexpr bool scaled = false; };
 
+// Infinities and NaN are kept as they are by any scale: finite values alone
+// decide it.
+__device__ __forceinline__ float finite_max(float m, float v) {
+  const float a = fabsf(v);
+  return a < INFINITY ? fmaxf(m, a) : m;
+}
+
 // 2^k that brings the largest magnitude into [2^13, 2^14) of f16; 1 where
-// there is none, or an infinity.
+// there is none.
 __device__ __forceinline__ float kept_scale_of(float amax) {
   const int e = (int)(__float_as_uint(amax) >> 23);            // biased exponent, amax >= 0
-  if (amax == 0.0f || e == 255) return 1.0f;
+  if (amax == 0.0f) return 1.0f;
   const int k = 13 + 127 - e;                                  // -114 .. 140
   return __uint_as_float((uint32_t)(min(max(k, -126), 126) + 127) << 23);
 }
@@ -391,8 +398,8 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
               v[c + j] = __float_as_uint(fa);
               v[64 + c + j] = __float_as_uint(f.act);
               if (Kept<T>::scaled) {
-                amax_a = fmaxf(amax_a, fabsf(fa));
-                amax_b = fmaxf(amax_b, fabsf(f.act));
+                amax_a = finite_max(amax_a, fa);
+                amax_b = finite_max(amax_b, f.act);
               }
             }
           } else {

@@ -269,6 +269,34 @@ def test_negative_tail_is_relative(cuda_ready, m, act, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("recompute", [False, True])
+def test_infinite_neighbour_of_finite_gradients(cuda_ready, recompute):
+    """One infinite column of a group of 64: the other columns' gradients stay
+    what they are, large and small (bf16 keeps 64 columns under one scale)."""
+    f = 128
+    p = {"x": torch.zeros(1, 8), "w_gate": torch.zeros(f, 8), "w_up": torch.zeros(f, 8),
+         "b_gate": torch.zeros(f), "b_up": torch.zeros(f), "dh": torch.ones(1, f)}
+    p["x"][0, 0] = 1.0
+    p["w_gate"][:, 0] = 3.0
+    p["w_up"][:, 0] = 2.0 ** 18
+    p["w_up"][1::2, 0] = 2.0 ** -3
+    p["w_up"][5, 0] = float("inf")
+    p = {n: v.bfloat16() for n, v in p.items()}
+    h, grads = run(p, recompute=recompute)
+    s = torch.sigmoid(torch.tensor(3.0, dtype=torch.float64))
+    dg = p["w_up"][:, 0].double() * s * (1 + 3 * (1 - s))
+    # the largest finite value of the group is 2^18, so 2^-3 is 21 powers of two
+    # below it and still a normal f16: half a step of f16, then of bf16
+    for name, want in (("b_gate", dg), ("w_gate", dg), ("b_up", torch.full((f,), float(3 * s)).double())):
+        got = grads[name].double().cpu()
+        got = got[:, 0] if got.dim() == 2 else got
+        others = [i for i in range(f) if i != 5]
+        off = (got - want).abs()[others]
+        assert (off <= want[others].abs() * (2 * 2.0 ** -8 + 2.0 ** -11 + 200 * U)).all(), name
+    assert torch.isinf(grads["b_gate"][5]) and torch.isinf(h[0, 5])
+
+
+@pytest.mark.gpu
 def test_no_rows(cuda_ready):
     p = make(0, 64, 128, torch.bfloat16, bias=True)
     h, g = run(p)
