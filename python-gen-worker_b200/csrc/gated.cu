@@ -18,15 +18,17 @@
 //            b = act(g), all that dg = dh a and du = dh b need of it.
 //   DGATE    the same tile again for a caller that kept nothing; the epilogue
 //            reads dh and writes dg and du (rounded to the operand type: they
-//            are tensor-core operands next).
+//            are tensor-core operands next) and, for the bias gradients, the
+//            column sums of each 32 rows before that rounding.
 //   DX       dg Wg + du Wu as one chain of K = 2 F into one accumulator.
 //   DW       dg^T x and du^T x, K = M.
 //
-// Accumulators, activations and column sums are f32; every output is rounded
-// once. a and b are kept with three bits or more beyond the operand type's, so
-// that keeping them adds next to nothing to the rounding of dg and du: for bf16
-// as f16 times a power of two per row and 64 columns (4 bytes a pair), for f16
-// as f32.
+// Accumulators, activations and column sums are f32. h and the bias gradients
+// are rounded once; so are dx and dW, from products whose operands dg and du
+// were rounded to 16 bits. a and b are kept with three bits or more beyond the
+// operand type's, so that keeping them adds next to nothing to the rounding of
+// dg and du: for bf16 as f16 times a power of two per row and 64 columns (4
+// bytes a pair), for f16 as f32.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <algorithm>
@@ -78,7 +80,8 @@ struct Args {
   void* kept; float* kept_scale;      // SAVE: a and b, planes [2][M][F], and their scales
   int tiles_m, tiles_n, half0, ntiles;
   // DX, DW with few tiles: each tile's K is split into `parts` of `part_k`
-  // k-blocks, and part p's f32 tile goes to partial + p * part_stride
+  // k-blocks, and part p's f32 tile goes to partial + p * part_stride. DGATE:
+  // column sums [2][M / 32 rounded up][F], or null
   int parts, part_k; float* partial; int64_t part_stride;
 };
 
@@ -218,6 +221,23 @@ __device__ __forceinline__ void patch_store(const uint8_t* patch, int lane, K* d
     if (r < rows && piece * N < cols) *reinterpret_cast<uint4*>(dst + r * ld + piece * N) = v;
   }
   __syncwarp();
+}
+
+// A warp's 32 rows (one a lane) of 32 columns, added up by column in 31
+// shuffles: each step halves the columns a lane carries. Returns the sum of
+// column `lane`; fixed order.
+__device__ __forceinline__ float column_sums(float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int half = 16; half; half /= 2) {
+    const bool up = lane & half;
+#pragma unroll
+    for (int k = 0; k < half; ++k) {
+      const float keep = up ? v[k + half] : v[k], give = up ? v[k] : v[k + half];
+      v[k] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+    }
+  }
+  return v[0];
 }
 
 template <int MODE, int ACT, typename T>
@@ -364,7 +384,9 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
       if constexpr (PROJ) {
         const int n0 = t.n0 + 64 * side, rows = a.M - row0, cols = a.F - n0;
         if (rows <= 0 || cols <= 0) continue;
-        if (MODE != SAVE && row >= a.M) continue;      // SAVE's lanes store for each other
+        // SAVE's lanes store for each other, DGATE's add up columns together
+        if (MODE == FORWARD && row >= a.M) continue;
+        const bool live = row < a.M;
         float amax_a = 0.0f, amax_b = 0.0f;
 #pragma unroll
         for (int c = 0; c < 64; c += 8) {
@@ -403,16 +425,18 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
               }
             }
           } else {
-            load8(static_cast<const T*>(a.dh) + (size_t)row * a.dhs + n0 + c, p);
+            if (live) load8(static_cast<const T*>(a.dh) + (size_t)row * a.dhs + n0 + c, p);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const ActValue f = activation<ACT, true>(g[j]);
-              o[j] = p[j] * u[j] * f.slope;
-              p[j] *= f.act;
+              o[j] = live ? p[j] * u[j] * f.slope : 0.0f;
+              p[j] = live ? p[j] * f.act : 0.0f;
+              v[c + j] = __float_as_uint(o[j]);
+              v[64 + c + j] = __float_as_uint(p[j]);
             }
-            store8(static_cast<T*>(a.o1) + (size_t)row * a.F + n0 + c, p);
+            if (live) store8(static_cast<T*>(a.o1) + (size_t)row * a.F + n0 + c, p);
           }
-          if (MODE != SAVE || row < a.M)
+          if (live)
             store8(static_cast<T*>(a.o0) + (size_t)row * a.F + n0 + c, o);
         }
         if constexpr (MODE == SAVE) {
@@ -441,7 +465,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
           };
           const float sa = Kept<T>::scaled ? kept_scale_of(amax_a) : 1.0f;
           const float sb = Kept<T>::scaled ? kept_scale_of(amax_b) : 1.0f;
-          if (Kept<T>::scaled && row < a.M) {
+          if (Kept<T>::scaled && live) {
             const int groups = (a.F + 63) / 64;
             a.kept_scale[(size_t)row * groups + n0 / 64] = sa;
             a.kept_scale[((size_t)a.M + row) * groups + n0 / 64] = sb;
@@ -449,6 +473,21 @@ gated_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CU
           K* ka = static_cast<K*>(a.kept) + (size_t)row0 * a.F + n0;
           put(ka, 0, sa);
           put(ka + (size_t)a.M * a.F, 64, sb);
+        }
+        if (MODE == DGATE && a.partial) {
+          // column sums of the warp's 32 rows, before dg and du were rounded
+          const int groups = (a.M + 31) / 32;
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 128; c += 32) {
+            float s[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[j] = __uint_as_float(v[c + j]);
+            const float sum = column_sums(s);
+            const int col = c % 64 + lane;
+            if (col < cols)
+              a.partial[((size_t)(c / 64) * groups + row0 / 32) * a.F + n0 + col] = sum;
+          }
         }
       } else {
         const int total = MODE == DX ? a.M : a.F, n0 = t.n0 + 128 * side;
@@ -664,12 +703,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tX, const __grid_constant__ 
 }
 
 // ------------------------------------------------- dg, du and bias gradients
-// From kept a and b (KEPT): dg = dh a, du = dh b, 256 columns a CTA (eight a
-// lane), its warps taking rows of one chunk in turn; with `partial`, the
-// column sums of what was written, joined in a fixed order by
-// column_join_kernel: partials [2][chunks][F]. Without KEPT (dg and du come
-// from the DGATE tiles) the sums alone.
-template <typename T, bool KEPT>
+// From kept a and b: dg = dh a, du = dh b, 256 columns a CTA (eight a lane),
+// its warps taking rows of one chunk in turn; with `partial`, the column sums
+// [2][chunks][F] of the products before they are rounded, for
+// column_join_kernel.
+template <typename T>
 __global__ void __launch_bounds__(256)
 gradients_kernel(const T* __restrict__ dh, int64_t dhs, const void* __restrict__ kept,
                  const float* __restrict__ scale, T* __restrict__ dg, T* __restrict__ du, int M,
@@ -686,40 +724,29 @@ gradients_kernel(const T* __restrict__ dh, int64_t dhs, const void* __restrict__
 #pragma unroll 2
     for (int r = r0 + warp; r < r1; r += 8) {
       const size_t at = (size_t)r * F + c0;
-      float g[8], u[8];
-      if constexpr (KEPT) {
-        float d[8], ra = 1.0f, rb = 1.0f;
-        load8(dh + (size_t)r * dhs + c0, d);
-        const K* ka = static_cast<const K*>(kept) + at;
-        if constexpr (Kept<T>::scaled) {
-          load8(ka, g);
-          load8(ka + plane, u);
-          // the scales are powers of two: their reciprocals are exact
-          ra = 1.0f / __ldg(scale + (size_t)r * groups + c0 / 64);
-          rb = 1.0f / __ldg(scale + ((size_t)M + r) * groups + c0 / 64);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            *reinterpret_cast<float4*>(g + j) = *reinterpret_cast<const float4*>(ka + j);
-            *reinterpret_cast<float4*>(u + j) = *reinterpret_cast<const float4*>(ka + plane + j);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          g[j] = d[j] * (g[j] * ra);
-          u[j] = d[j] * (u[j] * rb);
-        }
-        const uint4 rg = round8<T>(g), ru = round8<T>(u);
-        *reinterpret_cast<uint4*>(dg + at) = rg;
-        *reinterpret_cast<uint4*>(du + at) = ru;
-        if (partial) {
-          load8(reinterpret_cast<const T*>(&rg), g);
-          load8(reinterpret_cast<const T*>(&ru), u);
-        }
+      float g[8], u[8], d[8], ra = 1.0f, rb = 1.0f;
+      load8(dh + (size_t)r * dhs + c0, d);
+      const K* ka = static_cast<const K*>(kept) + at;
+      if constexpr (Kept<T>::scaled) {
+        load8(ka, g);
+        load8(ka + plane, u);
+        // the scales are powers of two: their reciprocals are exact
+        ra = 1.0f / __ldg(scale + (size_t)r * groups + c0 / 64);
+        rb = 1.0f / __ldg(scale + ((size_t)M + r) * groups + c0 / 64);
       } else {
-        load8(dg + at, g);
-        load8(du + at, u);
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          *reinterpret_cast<float4*>(g + j) = *reinterpret_cast<const float4*>(ka + j);
+          *reinterpret_cast<float4*>(u + j) = *reinterpret_cast<const float4*>(ka + plane + j);
+        }
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g[j] = d[j] * (g[j] * ra);
+        u[j] = d[j] * (u[j] * rb);
+      }
+      store8(dg + at, g);
+      store8(du + at, u);
       if (partial) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) { sg[j] += g[j]; su[j] += u[j]; }
@@ -759,14 +786,25 @@ parts_join_kernel(const float* __restrict__ partial, int parts, int64_t stride, 
   store8(i < n0 ? out0 + i : out1 + (i - n0), t);
 }
 
+// Bias gradients from column sums [2][chunks][F]: 32 columns a CTA, its eight
+// warps taking chunks in turn, joined in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(256)
 column_join_kernel(const float* __restrict__ partial, int chunks, int F, T* dbg, T* dbu) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  __shared__ float acc[8][32];
   T* out = blockIdx.y ? dbu : dbg;
-  if (c >= F || out == nullptr) return;
+  if (out == nullptr) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane;
   float t = 0.0f;
-  for (int k = 0; k < chunks; ++k) t += partial[((size_t)blockIdx.y * chunks + k) * F + c];
+  if (c < F)
+#pragma unroll 4
+    for (int k = warp; k < chunks; k += 8) t += partial[((size_t)blockIdx.y * chunks + k) * F + c];
+  acc[warp][lane] = t;
+  __syncthreads();
+  if (warp || c >= F) return;
+  t = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) t += acc[w][lane];
   out[c] = from_f32<T>(t);
 }
 
@@ -914,8 +952,11 @@ inline int64_t partial_bytes(const Split& s, int64_t elements) {
   return s.parts > 1 ? s.parts * elements * 4 : 0;
 }
 
+// Column sums of the bias gradients: of each 32 rows of the DGATE tiles, or
+// (a and b kept) of gradients_kernel's chunks, which are no more.
+inline int bias_groups(int M) { return cdiv(M, 32); }
 inline int64_t bias_bytes(int M, int F) {
-  return ((int64_t)2 * bias_chunks(M, F) * F * 4 + 255) / 256 * 256;
+  return ((int64_t)2 * bias_groups(M) * F * 4 + 255) / 256 * 256;
 }
 
 template <typename T>
@@ -938,17 +979,18 @@ int backward(const GatedBackward& w, cudaStream_t st) {
   Args a{};
   a.bg = w.bg; a.bu = w.bu; a.dh = w.dh; a.dhs = w.dhs; a.o0 = dg; a.o1 = du;
   a.M = M; a.D = D; a.F = F; a.act = w.act;
-  const int chunks = bias_chunks(M, F);
+  const int chunks = w.kept ? bias_chunks(M, F) : bias_groups(M);
   const bool bias = w.dbg || w.dbu;
-  const dim3 grid(cdiv(F, 256), chunks);
   if (int rc = bind_context()) return rc;
   if (w.kept) {
-    gradients_kernel<T, true><<<grid, 256, 0, st>>>(
+    gradients_kernel<T><<<dim3(cdiv(F, 256), chunks), 256, 0, st>>>(
         static_cast<const T*>(w.dh), w.dhs, w.kept, kept_scales<T>(w.kept, M, F),
         static_cast<T*>(dg), static_cast<T*>(du), M, F, cdiv(M, chunks), bias ? partial : nullptr);
     if (int rc = launch_status()) return rc;
   } else {
-    if (int rc = projections<T>(DGATE, w.x, w.xs, w.wg, w.wu, a, st)) return rc;
+    Args d = a;
+    d.partial = bias ? partial : nullptr;
+    if (int rc = projections<T>(DGATE, w.x, w.xs, w.wg, w.wu, d, st)) return rc;
   }
   if (w.dx) {
     CUtensorMap ag, au, bgm, bum;
@@ -995,13 +1037,7 @@ int backward(const GatedBackward& w, cudaStream_t st) {
       if (int rc = join<T>(c, w.dwg ? (int64_t)F * D : 0, c.part_stride, st)) return rc;
   }
   if (bias) {
-    if (!w.kept) {
-      gradients_kernel<T, false><<<grid, 256, 0, st>>>(nullptr, 0, nullptr, nullptr,
-                                                       static_cast<T*>(dg), static_cast<T*>(du), M,
-                                                       F, cdiv(M, chunks), partial);
-      if (int rc = launch_status()) return rc;
-    }
-    column_join_kernel<T><<<dim3(cdiv(F, 256), 2), 256, 0, st>>>(
+    column_join_kernel<T><<<dim3(cdiv(F, 32), 2), 256, 0, st>>>(
         partial, chunks, F, static_cast<T*>(w.dbg), static_cast<T*>(w.dbu));
     return launch_status();
   }

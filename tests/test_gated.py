@@ -297,6 +297,32 @@ def test_infinite_neighbour_of_finite_gradients(cuda_ready, recompute):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("recompute", [False, True])
+@pytest.mark.parametrize("m", [2, 34, 300])
+def test_bias_gradients_add_unrounded_terms(cuda_ready, m, recompute, dtype):
+    """Bias gradients are f32 sums of f32 dg and du, rounded once: rows in pairs
+    of opposite dh, so that a rounding of each term to the operand type would
+    show beside sums that nearly cancel. Only what bf16 keeps (f16 values) is
+    rounded before."""
+    p = make(m, 64, 392, dtype, seed=m, bias=True)
+    p["x"][1::2] = p["x"][0::2] + (torch.randn(m // 2, 64, generator=torch.Generator().manual_seed(1))
+                                   * 0.02).to(dtype)
+    p["dh"][1::2] = -p["dh"][0::2]
+    h, grads = run(p, "silu", ["b_gate", "b_up"], recompute=recompute)
+    r = {n: p[n].double().requires_grad_(True) for n in ("b_gate", "b_up")}
+    h64, g64, u64 = gated64(p["x"], p["w_gate"], p["w_up"], r["b_gate"], r["b_up"], "silu")
+    terms = dict(zip(r, torch.autograd.grad(h64, [g64, u64], p["dh"].double(), retain_graph=True)))
+    want = dict(zip(r, torch.autograd.grad(h64, list(r.values()), p["dh"].double())))
+    mag = gated_magnitudes(p["x"], p["w_gate"], p["w_up"], p["b_gate"], p["b_up"], p["dh"],
+                           (h64.detach(), g64.detach(), u64.detach()))
+    kept = half_step(torch.float16) if dtype == torch.bfloat16 and not recompute else 0.0
+    for n, e in (("b_gate", mag["dg"]), ("b_up", mag["du"])):
+        term = terms[n].abs() + e
+        check(grads[n], want[n], (e + (kept + (m + 2) * U) * term).sum(0), 1 / U, n)
+
+
+@pytest.mark.gpu
 def test_no_rows(cuda_ready):
     p = make(0, 64, 128, torch.bfloat16, bias=True)
     h, g = run(p)
