@@ -29,9 +29,14 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     all float16 -> h [..., F], contiguous. D and F are multiples of 8; weights
     and biases contiguous and 16-byte aligned (halves of a fused weight are).
     x may be a slice of wider rows; rows that 16-byte loads cannot step
-    through are copied first. f32 accumulation, one rounding. Differentiable
-    once in all of them. Where a gradient is wanted, 4 bytes per element of h
-    (bfloat16; 8 for float16) are kept for the backward pass, or, with
+    through are copied first. f32 accumulation; h is rounded once.
+
+    Differentiable once in all of them. The gradients of g and u are rounded to
+    x's type, as operands of the products that give the gradients of x and the
+    weights (a float16 one over 65504 is infinite there: scale the loss); the
+    bias gradients add them in f32. Where a gradient is wanted, 4 bytes per
+    element of h (bfloat16: act(g) and u act'(g) as scaled float16; 8 for
+    float16, as float32) are kept for the backward pass, or, with
     ``recompute``, nothing, and it computes the projections again."""
     code = ACTIVATIONS.get(activation)
     if code is None:
