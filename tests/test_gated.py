@@ -327,15 +327,18 @@ def test_f16_products_of_large_gradients_stay_in_their_rows(cuda_ready):
     """dg and du are float16 operands of the next products: a dg over 65504 is
     infinite there, in its own row of dx and its own row of dw_gate."""
     p = make(140, 64, 72, torch.float16)
-    p["dh"][7, 9], p["x"][7] = 60000.0, p["x"][7] * 4
-    h, grads = run(p)
+    p["x"][7] *= 4
     h64, g64, _ = gated64(*(p[n].double().requires_grad_(n == "x") for n in ("x", "w_gate", "w_up")),
                           None, None, "silu")
-    assert float(torch.autograd.grad(h64, g64, p["dh"].double())[0][7, 9].abs()) > 1e5
+    slope, = torch.autograd.grad(h64.sum(), g64)       # dg of a unit dh
+    f = int(slope[7].abs().argmax())
+    p["dh"][7, f] = 60000.0
+    assert float(slope[7, f].abs()) * 60000 > 1e5
+    h, grads = run(p)
     bad = torch.isfinite(grads["x"]).logical_not()
     assert bad[7].any() and not bad[torch.arange(140) != 7].any()
     bad = torch.isfinite(grads["w_gate"]).logical_not()
-    assert bad[9].any() and not bad[torch.arange(72) != 9].any()
+    assert bad[f].any() and not bad[torch.arange(72) != f].any()
 
 
 @pytest.mark.gpu
