@@ -11,7 +11,9 @@
 //   db = sum_samples (1 + s) S1
 // so one pass over x and dy feeds every gradient. Statistics and sums are f32
 // throughout (mean first, then the centred squares, both from registers);
-// each output is rounded once.
+// each output is rounded once. The row sum is divided by D: the product with a
+// rounded 1 / D can miss the mean of a row of one value by an ulp, which a
+// small eps turns into a z far from zero.
 //
 // HBM bounds both directions: x in and y out forward, x and dy in and dx out
 // backward. Column sums go through per-CTA partials and a second kernel in a
@@ -285,7 +287,7 @@ forward_kernel(const FwdArgs a, const FwdPlan p) {
         __syncwarp();
         if (lane == 0 && s + p.stages < steps) fill(s + p.stages);
       }
-      const float mean = lanes_sum<L>(sum2(acc)) * inv_d;
+      const float mean = lanes_sum<L>(sum2(acc)) / (float)a.D;
       const F2 neg = f2(-mean, -mean);
       acc = f2(0.0f, 0.0f);
       if constexpr (VECTOR) {
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(512) forward_block_kernel(const FwdArgs a) {
       sum += v[c][j];
     }
   const float inv_d = 1.0f / (float)a.D;
-  const float mean = block_sum(sum, red[0]) * inv_d;
+  const float mean = block_sum(sum, red[0]) / (float)a.D;
   float sq = 0.0f;
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(512) forward_pairs_kernel(const FwdArgs a) {
 #pragma unroll
     for (int j = 0; j < P; ++j) acc = add2(acc, v[c][j]);
   }
-  const float mean = total(acc, 0) * inv_d;
+  const float mean = total(acc, 0) / (float)a.D;
   const F2 neg = f2(-mean, -mean);
   acc = f2(0.0f, 0.0f);
 #pragma unroll
@@ -531,7 +533,7 @@ __global__ void __launch_bounds__(1024) forward_wide_kernel(const FwdArgs a) {
   float sum = 0.0f;
   for (int c = threadIdx.x; c < a.D; c += blockDim.x) sum += to_f32<T>(x[c]);
   const float inv_d = 1.0f / (float)a.D;
-  const float mean = block_sum(sum, red[0]) * inv_d;
+  const float mean = block_sum(sum, red[0]) / (float)a.D;
   float sq = 0.0f;
   for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
     const float d = to_f32<T>(x[c]) - mean;

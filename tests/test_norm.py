@@ -166,6 +166,35 @@ def test_constant_rows_far_means_and_bad_values(cuda_ready, dtype):
     assert torch.isnan(y[3]).all() and torch.isnan(y[4]).all()
 
 
+# widths whose rounded reciprocal times the row sum misses the mean of a row of 200
+INEXACT = [56, 61, 112, 190, 240, 504, 760, 1000, 1427, 1520, 1784, 2040, 2741, 3040, 3584, 3119,
+           5480, 5507, 5792, 10952]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", INEXACT)
+def test_rows_of_one_value_are_their_own_mean(cuda_ready, d):
+    """The sum of d values of 200 is exact in f32 (200 d < 2^24), so its quotient
+    by d is 200 and z is zero: few rows and many, aligned and not."""
+    from gen_worker_b200 import layer_norm
+
+    for dtype in TYPES:
+        for rows in (3, 8400 if d < 4000 else 9):
+            y = layer_norm(torch.full((rows, d), 200.0, device="cuda", dtype=dtype))
+            assert not y.any(), (dtype, rows)
+        wide = torch.full((5, d + 1), 200.0, device="cuda", dtype=dtype)
+        assert not layer_norm(wide[:, 1:]).any(), (dtype, "unaligned")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [96, 320, 1280, 1153])
+def test_gradients_of_rows_far_from_zero(cuda_ready, d, dtype):
+    p = make((70, d), dtype, seed=d, affine=True)
+    p["x"] = (p["x"].float() + 200.0 * torch.linspace(-1, 1, 70)[:, None]).to(dtype)
+    run_and_check(p)
+
+
 @pytest.mark.gpu
 def test_expanded_gradient_and_broadcast_modulation(cuda_ready):
     """A gradient of stride 0, and one modulation row expanded over the batch."""
