@@ -984,55 +984,82 @@ struct SumArgs {
   void* dw; void* db; void* ds; void* dt;      // any may be null
 };
 
-// Sums the partials over each sample's chunks: 32 columns a CTA, its 16 warps
-// taking chunks in turn, joined in a fixed order. One sample per blockIdx.y,
-// or (weight gradients wanted) all samples in turn.
+// Sums the partials, 32 columns a CTA, its 16 warps joined in a fixed order.
+// blockIdx.y takes samples in turn for dscale and dshift, its warps a sample's
+// chunks; with weight gradients wanted, the last blockIdx.y takes all samples'
+// chunks at once for them, each times its sample's 1 + s. Runs of 64 terms are
+// added up before they join a thread's total, so many samples lose no more
+// bits than few.
 template <typename T>
 __global__ void __launch_bounds__(512) sums_kernel(const SumArgs a) {
   __shared__ float acc[2][16][33];
+  constexpr int WARPS = 16, RUN = 64;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  const bool all = gridDim.y == 1;
-  float dw = 0.0f, db = 0.0f;
-  for (int64_t smp = blockIdx.y; smp < a.samples; smp += gridDim.y) {
+  // the warps' sums, joined, in warp 0
+  const auto join = [&](float& u, float& v) {
+    acc[0][w][lane] = u;
+    acc[1][w][lane] = v;
+    __syncthreads();
+    if (w == 0) {
+      u = v = 0.0f;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) { u += acc[0][k][lane]; v += acc[1][k][lane]; }
+    }
+  };
+  const bool weights = a.dw || a.db;
+  if (weights && blockIdx.y == gridDim.y - 1) {
+    const uint32_t total = (uint32_t)(a.samples * a.chunks);   // at most 2^31
+    float dw = 0.0f, db = 0.0f;
+    if (c < a.D)
+      for (uint32_t i0 = w; i0 < total; i0 += WARPS * RUN) {
+        const uint32_t end = min(total, i0 + WARPS * RUN);
+        float rw = 0.0f, rb = 0.0f;
+#pragma unroll 4
+        for (uint32_t i = i0; i < end; i += WARPS) {
+          const float* p = a.partial + i * 2 * (int64_t)a.D + c;
+          float s[1], up = 1.0f;
+          if (a.s.p) { load_param<T, 1>(a.s, i / (uint32_t)a.chunks, c, s); up += s[0]; }
+          rb += up * __ldg(p);
+          rw += up * __ldg(p + a.D);
+        }
+        dw += rw;
+        db += rb;
+      }
+    join(dw, db);
+    if (w == 0 && c < a.D) {
+      const auto put = [&](void* o, float v) {
+        if (a.w.f32) static_cast<float*>(o)[c] = v;
+        else static_cast<T*>(o)[c] = from_f32<T>(v);
+      };
+      if (a.dw) put(a.dw, dw);
+      if (a.db) put(a.db, db);
+    }
+    return;
+  }
+  const int rows = gridDim.y - weights;
+  for (int64_t smp = blockIdx.y; smp < a.samples; smp += rows) {
     float s1 = 0.0f, s2 = 0.0f;
     if (c < a.D)
-      for (int k = w; k < a.chunks; k += 16) {
+      for (int k = w; k < a.chunks; k += WARPS) {
         const float* p = a.partial + (smp * a.chunks + k) * 2 * (int64_t)a.D + c;
         s1 += __ldg(p);
         s2 += __ldg(p + a.D);
       }
-    acc[0][w][lane] = s1;
-    acc[1][w][lane] = s2;
-    __syncthreads();
+    join(s1, s2);
     if (w == 0 && c < a.D) {
-      s1 = s2 = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) { s1 += acc[0][k][lane]; s2 += acc[1][k][lane]; }
-      float p[1], up = 1.0f;
-      if (a.s.p) { load_param<T, 1>(a.s, smp, c, p); up += p[0]; }
-      dw += up * s2;
-      db += up * s1;
-      const auto put = [&](void* o, int f32, float v) {
-        if (f32) static_cast<float*>(o)[smp * a.D + c] = v;
+      const auto put = [&](void* o, float v) {
+        if (a.s.f32) static_cast<float*>(o)[smp * a.D + c] = v;
         else static_cast<T*>(o)[smp * a.D + c] = from_f32<T>(v);
       };
-      if (a.dt) put(a.dt, a.s.f32, s1);
+      if (a.dt) put(a.dt, s1);
       if (a.ds) {
-        float v = s2;
+        float p[1], v = s2;
         if (a.w.p) { load_param<T, 1>(a.w, 0, c, p); v *= p[0]; }
         if (a.b.p) { load_param<T, 1>(a.b, 0, c, p); v += p[0] * s1; }
-        put(a.ds, a.s.f32, v);
+        put(a.ds, v);
       }
     }
     __syncthreads();
-  }
-  if (all && w == 0 && c < a.D) {
-    const auto put = [&](void* o, float v) {
-      if (a.w.f32) static_cast<float*>(o)[c] = v;
-      else static_cast<T*>(o)[c] = from_f32<T>(v);
-    };
-    if (a.dw) put(a.dw, dw);
-    if (a.db) put(a.db, db);
   }
 }
 
@@ -1220,9 +1247,9 @@ int backward_t(const BwdArgs& a, int64_t samples, const SumArgs& sums, bool want
       rc = backward_v<T, 1>(a, samples, st);
   }
   if (rc || !want_sums) return rc;
-  const bool all = sums.dw || sums.db;
-  const unsigned y = all ? 1u : (unsigned)(samples < 65535 ? samples : 65535);
-  sums_kernel<T><<<dim3((a.D + 31) / 32, y > 0 ? y : 1), 512, 0, st>>>(sums);
+  const unsigned y = (sums.ds || sums.dt ? (unsigned)std::min<int64_t>(samples, 65534) : 0u) +
+                     (sums.dw || sums.db ? 1u : 0u);
+  sums_kernel<T><<<dim3((a.D + 31) / 32, y), 512, 0, st>>>(sums);
   return launch_status();
 }
 

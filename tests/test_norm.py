@@ -196,6 +196,24 @@ def test_gradients_of_rows_far_from_zero(cuda_ready, d, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [8, 40, 264])
+def test_column_sums_over_many_samples(cuda_ready, d):
+    """A modulation row for each of 40000 rows: weight and bias gradients add
+    40000 samples. dy = 1 + 2^-10 loses its last bit in every step of one long
+    f32 sum; chains of at most 64 terms, joined in turn, keep it. The bound is
+    the column sums' usual count, 200 roundings of the magnitudes."""
+    rows = 40000
+    g = torch.Generator().manual_seed(d)
+    p = {"x": torch.randn(rows, d, generator=g), "weight": torch.ones(d), "bias": torch.zeros(d),
+         "scale": torch.zeros(rows, d), "shift": torch.zeros(rows, d),
+         "dy": torch.full((rows, d), 1 + 2.0 ** -10)}
+    run_and_check(p)
+    p["scale"] = torch.randn(rows, d, generator=g) * 0.3
+    p["dy"] = torch.randn(rows, d, generator=g)
+    run_and_check(p, names=["weight", "scale"])
+
+
+@pytest.mark.gpu
 def test_expanded_gradient_and_broadcast_modulation(cuda_ready):
     """A gradient of stride 0, and one modulation row expanded over the batch."""
     from gen_worker_b200 import layer_norm
