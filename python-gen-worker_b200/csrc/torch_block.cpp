@@ -70,6 +70,15 @@ void refuse_second_order(const char* what, const Ts&... ts) {
   TORCH_CHECK(!any, what, " has no second derivative (create_graph=True)");
 }
 
+// Below the Autograd key no tangent is looked at: a dual tensor of forward-mode
+// differentiation would lose its own without a word.
+bool tangent_of(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool tangent_of(const OptTensor& t) { return has(t) && tangent_of(*t); }
+template <typename... Ts>
+void refuse_tangents(const char* what, const Ts&... ts) {
+  NEED(!(tangent_of(ts) || ...), what, " has no forward-mode derivative: use reverse mode");
+}
+
 // While a graph that used a leaf lives, torch keeps that leaf's gradient on the
 // stream of that graph. A backward pass captured on another stream would have
 // to wait for it across the capture, which breaks the capture in the middle of
@@ -305,6 +314,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 
 Tensor layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b,
                            const OptTensor& scale, const OptTensor& shift, double eps) {
+  refuse_tangents("layer_norm", x, w, b, scale, shift);
   if (at::GradMode::is_enabled() &&
       (wants(x) || wants(w) || wants(b) || wants(scale) || wants(shift))) {
     refuse_foreign_leaves("layer_norm", x, w, b, scale, shift);
@@ -506,6 +516,7 @@ std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptTensor& k,
                                            const Tensor& positions, const Tensor& inv_freq,
                                            const OptTensor& axis, bool interleaved, double scale,
                                            bool inverse) {
+  refuse_tangents("rotary", q, k, positions, inv_freq);
   if (at::GradMode::is_enabled() && (wants(q) || wants(k))) {
     refuse_foreign_leaves("rotary", q, k);
     auto r = RotaryFn::apply(q, k, positions, inv_freq, axis, interleaved, scale, inverse);
@@ -519,6 +530,7 @@ std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptTensor& k,
 void rotary_inplace_autograd(Tensor q, const OptTensor& k, const Tensor& positions,
                              const Tensor& inv_freq, const OptTensor& axis, bool interleaved,
                              double scale, bool inverse) {
+  refuse_tangents("rotary_", q, k, positions, inv_freq);
   NEED(!(at::GradMode::is_enabled() && (wants(q) || wants(k))),
        "rotary_ writes in place and keeps no gradient: use rotary");
   {
@@ -691,6 +703,7 @@ struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
 Tensor gated_linear_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu,
                              const OptTensor& bg, const OptTensor& bu, int64_t act,
                              bool recompute) {
+  refuse_tangents("gated_linear", x, wg, wu, bg, bu);
   if (at::GradMode::is_enabled() &&
       (wants(x) || wants(wg) || wants(wu) || wants(bg) || wants(bu))) {
     refuse_foreign_leaves("gated_linear", x, wg, wu, bg, bu);

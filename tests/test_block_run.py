@@ -317,3 +317,74 @@ def test_fake_tensors_trace_through():
         q, k = gw.rotary(x.view(2, 5, 2, 32), None, torch.empty(5, device="cuda", dtype=torch.int64),
                          torch.empty(8, device="cuda", dtype=torch.float64))
         assert q.shape == (2, 5, 2, 32) and k is None
+
+
+def _fake_calls():
+    """Each operator on fake tensors: (call of its tensors, the tensors)."""
+    import gen_worker_b200 as gw
+
+    def new(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, device="cuda", dtype=dtype)
+
+    pos, inv = new(5, dtype=torch.int64), new(8, dtype=torch.float64)
+    return [
+        (lambda x, w, b, s, t: gw.layer_norm(x, w, b, scale=s, shift=t),
+         [new(2, 5, 64), new(64), new(64), new(2, 64), new(2, 64)]),
+        (lambda q, k: gw.rotary(q, k, pos, inv), [new(2, 5, 2, 32), new(2, 5, 1, 32)]),
+        (lambda x, a, b, c, d: gw.gated_linear(x, a, b, c, d),
+         [new(2, 5, 64), new(72, 64), new(72, 64), new(72), new(72)]),
+        (lambda x, a, b: gw.gated_linear(x, a, b, recompute=True),
+         [new(2, 5, 64), new(72, 64), new(72, 64)]),
+    ]
+
+
+def _dual_calls(calls):
+    """Calls with a tangent on one of their tensors, by forward_ad and by jvp."""
+    from torch.autograd import forward_ad
+
+    for call, tensors in calls:
+        for i in range(len(tensors)):
+            def dual(call=call, tensors=tensors, i=i):
+                with forward_ad.dual_level():
+                    mixed = list(tensors)
+                    mixed[i] = forward_ad.make_dual(tensors[i], torch.ones_like(tensors[i]))
+                    return call(*mixed)
+
+            yield dual
+
+
+def test_forward_mode_is_refused():
+    """A tangent on any input is refused, never dropped."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import gen_worker_b200 as gw
+    from gen_worker_b200.ops import SvdqB200Error
+
+    with FakeTensorMode():
+        calls = _fake_calls()
+        pos = torch.empty(5, device="cuda", dtype=torch.float32)
+        inv = torch.empty(8, device="cuda", dtype=torch.float64)
+        q = [torch.empty(2, 5, 2, 32, device="cuda") for _ in range(2)]
+        calls.append((lambda q, k, p, f: gw.rotary(q, k, p, f), [*q, pos, inv]))
+        calls.append((lambda q, k, p, f: gw.rotary_(q, k, p, f), [*q, pos, inv]))
+        for dual in _dual_calls(calls):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(SvdqB200Error, match="forward-mode"):
+                    dual()
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_on_the_gpu(cuda_ready):
+    import gen_worker_b200 as gw
+    from gen_worker_b200.ops import SvdqB200Error
+
+    x = torch.randn(4, 64, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(72, 64, device="cuda", dtype=torch.bfloat16)
+    rope = gw.RotaryEmbedding(16, device="cuda")
+    pos = torch.arange(4, device="cuda")
+    calls = [(lambda x: gw.layer_norm(x), [x]), (lambda x, w: gw.gated_linear(x, w, w), [x, w]),
+             (lambda x: rope(x.view(4, 4, 16), None, pos), [x]),
+             (lambda x: rope.rotate_(x.view(4, 4, 16), None, pos), [x.clone()])]
+    for dual in _dual_calls(calls):
+        with pytest.raises(SvdqB200Error, match="forward-mode"):
+            dual()
