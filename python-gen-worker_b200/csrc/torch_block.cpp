@@ -512,11 +512,17 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
   }
 };
 
+void refuse_learned_angles(const Tensor& positions, const Tensor& inv_freq) {
+  NEED(!(at::GradMode::is_enabled() && (wants(positions) || wants(inv_freq))),
+       "positions and inv_freq get no gradient: pass them detached");
+}
+
 std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const OptTensor& k,
                                            const Tensor& positions, const Tensor& inv_freq,
                                            const OptTensor& axis, bool interleaved, double scale,
                                            bool inverse) {
   refuse_tangents("rotary", q, k, positions, inv_freq);
+  refuse_learned_angles(positions, inv_freq);
   if (at::GradMode::is_enabled() && (wants(q) || wants(k))) {
     refuse_foreign_leaves("rotary", q, k);
     auto r = RotaryFn::apply(q, k, positions, inv_freq, axis, interleaved, scale, inverse);
@@ -531,6 +537,7 @@ void rotary_inplace_autograd(Tensor q, const OptTensor& k, const Tensor& positio
                              const Tensor& inv_freq, const OptTensor& axis, bool interleaved,
                              double scale, bool inverse) {
   refuse_tangents("rotary_", q, k, positions, inv_freq);
+  refuse_learned_angles(positions, inv_freq);
   NEED(!(at::GradMode::is_enabled() && (wants(q) || wants(k))),
        "rotary_ writes in place and keeps no gradient: use rotary");
   {

@@ -44,7 +44,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
     ``positions`` int64, int32 or float32: [S] or [B, S]; with ``axis`` (int32
     [rotary_dim / 2], the position axis of each pair) [S, A] or [B, S, A].
     ``inv_freq`` float64 [rotary_dim / 2]. Rotated features are multiplied by
-    ``scale``. Differentiable in q and k, to any order."""
+    ``scale``. Differentiable in q and k, to any order; positions and
+    frequencies that need a gradient are refused."""
     qo, ko = _call("rotary", q, k, positions, inv_freq, axis, interleaved, scale)
     return qo, None if k is None else ko
 

@@ -126,6 +126,26 @@ def test_strides(cuda_ready):
 
 
 @pytest.mark.gpu
+def test_learned_angles_are_refused(cuda_ready):
+    """No gradient reaches positions or frequencies: asking for one is an error,
+    not a silent zero."""
+    import gen_worker_b200 as gw
+    from gen_worker_b200.ops import SvdqB200Error
+
+    q = torch.randn(1, 3, 2, 16, device="cuda")
+    pos = torch.arange(3, device="cuda").float()
+    inv = gw.rotary_frequencies(16)[0].cuda()
+    for p, f in ((pos.clone().requires_grad_(True), inv), (pos, inv.clone().requires_grad_(True))):
+        for x in (q, q.clone().requires_grad_(True)):
+            with pytest.raises(SvdqB200Error, match="gradient"):
+                gw.rotary(x, None, p, f)
+        with pytest.raises(SvdqB200Error, match="gradient"):
+            gw.rotary_(q, None, p, f)
+        with torch.no_grad():
+            assert gw.rotary(q, None, p, f)[0].shape == q.shape
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_gradients(cuda_ready, dtype, interleaved):
