@@ -18,8 +18,10 @@
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <tuple>
+#include <vector>
 
 #include "../../include/gwb200.h"
 
@@ -429,29 +431,48 @@ std::tuple<Tensor, Tensor> rotary_cuda(const Tensor& q, const OptTensor& k,
   return {qo, ko};
 }
 
-// Whether two tensors of one storage can touch the same element: apart only
-// when their address ranges are, or when they step alike over batch and token
-// and their heads lie apart within one token (views of a fused projection).
-bool share_heads(const Tensor& q, const Tensor& k) {
+// Whether `gap` is the sum of one multiple of each term's stride within that
+// term's range. Terms come in order of falling stride, and what the later ones
+// can reach leaves few multiples of a term to try; a search that would try many
+// all the same (odd strides that mesh) says yes.
+struct Term { int64_t stride, low, high; };
+bool reaches(const Term* t, size_t n, int64_t gap, int* tries) {
+  if (n == 0) return gap == 0;
+  int64_t low = 0, high = 0;
+  for (size_t i = 1; i < n; ++i) {
+    low += t[i].low * t[i].stride;
+    high += t[i].high * t[i].stride;
+  }
+  const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  const int64_t first = std::max(t->low, -floor_div(high - gap, t->stride));
+  const int64_t last = std::min(t->high, floor_div(gap - low, t->stride));
+  for (int64_t m = first; m <= last; ++m)
+    if (--*tries < 0 || reaches(t + 1, n - 1, gap - m * t->stride, tries)) return true;
+  return false;
+}
+
+// Whether two tensors of one storage have an element in common: an index of
+// each whose offsets differ by their distance. A dimension of one stride in
+// both is one term, the difference of its two indices.
+bool share_elements(const Tensor& q, const Tensor& k) {
   if (!q.is_alias_of(k) || q.numel() == 0 || k.numel() == 0) return false;
-  const auto span = [](const Tensor& t) {
-    int64_t n = 1;
-    for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
-    return n;
+  std::vector<Term> terms;
+  const auto add = [&](int64_t stride, int64_t low, int64_t high) {
+    if (stride > 0 && low < high) terms.push_back({stride, low, high});
   };
-  const int64_t gap = k.storage_offset() - q.storage_offset();
-  if (gap >= span(q) || -gap >= span(k)) return false;
-  const int64_t h = q.dim() - 2;
-  for (int64_t d = 0; d < q.dim(); ++d)
-    if (d != h && q.size(d) > 1 && q.stride(d) != k.stride(d)) return true;
-  const auto heads = [&](const Tensor& t) { return (t.size(h) - 1) * t.stride(h) + t.size(-1); };
-  // one token's heads of both, apart and inside the step to the next token
-  int64_t step = -1;
-  for (int64_t d = 0; d < h; ++d)
-    if (q.size(d) > 1 && (step < 0 || q.stride(d) < step)) step = q.stride(d);
-  const bool apart = gap >= 0 ? gap >= heads(q) && (step < 0 || gap + heads(k) <= step)
-                              : -gap >= heads(k) && (step < 0 || -gap + heads(q) <= step);
-  return !apart;
+  for (int64_t d = 0; d < q.dim(); ++d) {
+    const int64_t up = q.size(d) - 1, down = 1 - k.size(d);
+    if (q.stride(d) == k.stride(d)) {
+      add(q.stride(d), down, up);
+    } else {
+      add(q.stride(d), 0, up);
+      add(k.stride(d), down, 0);
+    }
+  }
+  std::sort(terms.begin(), terms.end(),
+            [](const Term& a, const Term& b) { return a.stride > b.stride; });
+  int tries = 10000;
+  return reaches(terms.data(), terms.size(), k.storage_offset() - q.storage_offset(), &tries);
 }
 
 void rotary_inplace_cuda(Tensor q, const OptTensor& k, const Tensor& positions,
@@ -469,7 +490,7 @@ void rotary_inplace_cuda(Tensor q, const OptTensor& k, const Tensor& positions,
   Tensor kt;
   if (has(k)) {
     writable(*k, "k");
-    NEED(!share_heads(q, *k), "q and k share memory and cannot both be rotated in place");
+    NEED(!share_elements(q, *k), "q and k share memory and cannot both be rotated in place");
     kt = *k;
   }
   rotary_call(r, q, q, k, &kt, positions, inv_freq, axis, interleaved, scale, inverse);

@@ -126,6 +126,57 @@ def test_strides(cuda_ready):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b,s,h,hk", [(1, 7, 4, 4), (2, 7, 4, 4), (3, 1, 4, 2), (2, 5, 2, 2),
+                                      (2, 9, 6, 2)])
+def test_in_place_in_common_layouts(cuda_ready, b, s, h, hk):
+    """q and k of one fused tensor with its dimensions in any order: they share
+    no element, so both are rotated where they lie."""
+    from gen_worker_b200 import RotaryEmbedding
+
+    rope = RotaryEmbedding(64, device="cuda")
+    pos = torch.arange(s, device="cuda") + 5
+    g = torch.Generator().manual_seed(b + s)
+    fused = torch.randn(b, s, h + 2 * hk, 64, generator=g)
+    for order in ((0, 1, 2, 3), (0, 2, 1, 3), (1, 0, 2, 3), (1, 2, 0, 3), (2, 0, 1, 3), (2, 1, 0, 3)):
+        back = [order.index(i) for i in range(4)]
+        base = fused.permute(order).contiguous().cuda()       # the layout in memory
+        view = base.permute(back)                             # as [B, S, heads, D]
+        q, k = view[:, :, :h], view[:, :, h:h + hk]
+        qo, ko = rope(q, k, pos)
+        rope.rotate_(q, k, pos)
+        assert torch.equal(q, qo) and torch.equal(k, ko), order
+        assert torch.equal(view[:, :, h + hk:].cpu(), fused[:, :, h + hk:])
+    mesh = fused.reshape(b, s, -1, 2, 64).cuda() if h == hk else None     # heads of q and k in turn
+    if mesh is not None:
+        q, k = mesh[:, :, :, 0], mesh[:, :, :, 1]
+        qo, ko = rope(q, k, pos)
+        rope.rotate_(q, k, pos)
+        assert torch.equal(q, qo) and torch.equal(k, ko)
+
+
+@pytest.mark.gpu
+def test_in_place_still_refuses_shared_elements(cuda_ready):
+    import gen_worker_b200 as gw
+    from gen_worker_b200.ops import SvdqB200Error
+
+    inv = gw.rotary_frequencies(16)[0].cuda()
+    pos = torch.arange(6, device="cuda")
+    base = torch.randn(2, 8, 6, 16, device="cuda")           # [B, heads, S, D]
+    flat = torch.randn(4000, device="cuda")
+    pairs = [
+        (base[:, :4].transpose(1, 2), base[:, 3:7].transpose(1, 2)),
+        (base[:1, :4].transpose(1, 2), base[:1, 3:4].transpose(1, 2)),
+        # k one feature behind q, and in steps that meet q's only now and then
+        (flat[:768].view(1, 6, 8, 16), flat[1:769].view(1, 6, 8, 16)),
+        (flat.as_strided((1, 6, 2, 16), (0, 100, 32, 1)),
+         flat.as_strided((1, 6, 2, 16), (0, 70, 32, 1), 16)),
+    ]
+    for q, k in pairs:
+        with pytest.raises(SvdqB200Error, match="share memory"):
+            gw.rotary_(q, k, pos, inv)
+
+
+@pytest.mark.gpu
 def test_learned_angles_are_refused(cuda_ready):
     """No gradient reaches positions or frequencies: asking for one is an error,
     not a silent zero."""
