@@ -9,7 +9,6 @@
 // Python wrappers turn it into the package's error); a backward pass asked to
 // build a graph of its own is refused.
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -475,6 +474,27 @@ bool share_elements(const Tensor& q, const Tensor& k) {
   return reaches(terms.data(), terms.size(), k.storage_offset() - q.storage_offset(), &tries);
 }
 
+// Whether two indices of one tensor name the same element: an expanded
+// dimension, or two indices whose first difference some later ones undo.
+bool overlaps_itself(const Tensor& t) {
+  if (t.numel() < 2 || t.is_non_overlapping_and_dense()) return false;
+  std::vector<Term> terms;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) < 2) continue;
+    if (t.stride(d) == 0) return true;
+    terms.push_back({t.stride(d), 1 - t.size(d), t.size(d) - 1});
+  }
+  std::sort(terms.begin(), terms.end(),
+            [](const Term& a, const Term& b) { return a.stride > b.stride; });
+  int tries = 10000;
+  for (size_t i = 0; i < terms.size(); ++i) {
+    Term& first = terms[i];
+    first.low = 1;
+    if (reaches(&first, terms.size() - i, 0, &tries)) return true;
+  }
+  return false;
+}
+
 void rotary_inplace_cuda(Tensor q, const OptTensor& k, const Tensor& positions,
                          const Tensor& inv_freq, const OptTensor& axis, bool interleaved,
                          double scale, bool inverse) {
@@ -483,7 +503,7 @@ void rotary_inplace_cuda(Tensor q, const OptTensor& k, const Tensor& positions,
   const auto writable = [](const Tensor& t, const char* name) {
     NEED(t.size(-1) <= 1 || t.stride(-1) == 1, name,
          " must be dense in its last dimension to be rotated in place");
-    NEED(at::has_internal_overlap(t) != at::MemOverlap::Yes, name,
+    NEED(!overlaps_itself(t), name,
          " overlaps itself and cannot be rotated in place");
   };
   writable(q, "q");

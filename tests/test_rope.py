@@ -177,6 +177,34 @@ def test_in_place_still_refuses_shared_elements(cuda_ready):
 
 
 @pytest.mark.gpu
+def test_in_place_refuses_a_tensor_over_itself(cuda_ready):
+    """Windows of one buffer that overlap are refused, those that only lie close
+    are rotated."""
+    import gen_worker_b200 as gw
+    from gen_worker_b200.ops import SvdqB200Error
+
+    inv = gw.rotary_frequencies(16)[0].cuda()
+    pos = torch.arange(6, device="cuda")
+    flat = torch.randn(4000, device="cuda")
+    over = [((1, 6, 2, 16), (0, 24, 16, 1)), ((2, 6, 2, 16), (100, 32, 16, 1)),
+            ((1, 6, 2, 16), (0, 0, 16, 1)), ((1, 6, 3, 16), (0, 32, 16, 1)),
+            ((1, 6, 2, 16), (0, 32, 15, 1)), ((2, 6, 2, 16), (176, 34, 17, 1))]
+    for size, stride in over:
+        with pytest.raises(SvdqB200Error, match="overlaps itself"):
+            gw.rotary_(flat.as_strided(size, stride), None, pos, inv)
+        with pytest.raises(SvdqB200Error, match="overlaps itself"):
+            gw.rotary_(torch.randn(size, device="cuda"), flat.as_strided(size, stride), pos, inv)
+    close = [((1, 6, 2, 16), (7, 32, 16, 1)), ((2, 6, 2, 16), (192, 32, 16, 1)),
+             ((2, 6, 2, 16), (32, 64, 16, 1)), ((2, 6, 2, 16), (16, 64, 32, 1)),
+             ((2, 6, 2, 16), (999, 17, 500, 1)), ((1, 1, 2, 16), (0, 3, 16, 1))]
+    for size, stride in close:
+        q = flat.as_strided(size, stride)
+        want, _ = gw.rotary(q, None, pos[:size[1]], inv)
+        gw.rotary_(q, None, pos[:size[1]], inv)
+        assert torch.equal(q, want), (size, stride)
+
+
+@pytest.mark.gpu
 def test_learned_angles_are_refused(cuda_ready):
     """No gradient reaches positions or frequencies: asking for one is an error,
     not a silent zero."""
