@@ -581,6 +581,16 @@ void rotary_inplace_autograd(Tensor q, const OptTensor& k, const Tensor& positio
   refuse_learned_angles(positions, inv_freq);
   NEED(!(at::GradMode::is_enabled() && (wants(q) || wants(k))),
        "rotary_ writes in place and keeps no gradient: use rotary");
+  at::AutoDispatchBelowAutograd below;
+  static auto op = op_of<decltype(rotary_inplace_cuda)>("gwb200::rotary_");
+  op.call(q, k, positions, inv_freq, axis, interleaved, scale, inverse);
+}
+
+// Counts the change where autograd looks for it. A key of its own: inference
+// mode passes the Autograd key by, but not this one, for tensors made outside it.
+void rotary_inplace_counted(Tensor q, const OptTensor& k, const Tensor& positions,
+                            const Tensor& inv_freq, const OptTensor& axis, bool interleaved,
+                            double scale, bool inverse) {
   {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = op_of<decltype(rotary_inplace_cuda)>("gwb200::rotary_");
@@ -793,6 +803,10 @@ TORCH_LIBRARY_IMPL(gwb200, CUDA, m) {
   m.impl("gated_linear", &gwb200_block::gated_linear_cuda);
   m.impl("gated_linear_keep", &gwb200_block::gated_linear_keep_cuda);
   m.impl("gated_linear_backward", &gwb200_block::gated_linear_backward_cuda);
+}
+
+TORCH_LIBRARY_IMPL(gwb200, ADInplaceOrView, m) {
+  m.impl("rotary_", &gwb200_block::rotary_inplace_counted);
 }
 
 TORCH_LIBRARY_IMPL(gwb200, Autograd, m) {

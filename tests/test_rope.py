@@ -205,6 +205,25 @@ def test_in_place_refuses_a_tensor_over_itself(cuda_ready):
 
 
 @pytest.mark.gpu
+def test_in_place_counts_as_a_change(cuda_ready):
+    """Autograd must see that a saved tensor was rotated, in inference mode too."""
+    from gen_worker_b200 import RotaryEmbedding
+
+    rope = RotaryEmbedding(16, device="cuda")
+    pos = torch.arange(3, device="cuda")
+    for mode in (torch.no_grad, torch.inference_mode):
+        q, k = (torch.randn(1, 3, 2, 16, device="cuda") for _ in range(2))
+        w = torch.randn(16, device="cuda", requires_grad=True)
+        y = (w * q).sum() + (w * k).sum()
+        with mode():
+            before = q._version, k._version
+            rope.rotate_(q, k, pos)
+            assert (q._version, k._version) == (before[0] + 1, before[1] + 1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+@pytest.mark.gpu
 def test_learned_angles_are_refused(cuda_ready):
     """No gradient reaches positions or frequencies: asking for one is an error,
     not a silent zero."""
