@@ -97,9 +97,21 @@ void refuse_foreign_leaf(const char* what, const Tensor& t) {
 void refuse_foreign_leaf(const char* what, const OptTensor& t) {
   if (has(t)) refuse_foreign_leaf(what, *t);
 }
+// A tensor that stands for one while a call is traced or transformed: there may
+// be no GPU, and nothing is captured.
+bool traced(const Tensor& t) {
+  return t.defined() &&
+         t.key_set().has_any(c10::DispatchKeySet(
+             {c10::DispatchKey::Python, c10::DispatchKey::Functionalize,
+              c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched}));
+}
+bool traced(const OptTensor& t) { return has(t) && traced(*t); }
 template <typename... Ts>
-void refuse_foreign_leaves(const char* what, const Ts&... ts) {
+void refuse_foreign_leaves(const char* what, const Tensor& x, const Ts&... ts) {
+  if (!x.is_cuda() || traced(x) || (traced(ts) || ...)) return;
+  const c10::cuda::CUDAGuard guard(x.device());
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  refuse_foreign_leaf(what, x);
   (refuse_foreign_leaf(what, ts), ...);
 }
 

@@ -338,6 +338,49 @@ def _fake_calls():
     ]
 
 
+def test_fake_tensors_trace_what_needs_gradients():
+    """The calls of a training step trace on a machine without a GPU, and the
+    backward ops' fakes give each gradient its parameter's shape and type. (The
+    autograd engine itself asks for the device: the whole pass runs below.)"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        for call, tensors in _fake_calls():
+            out = call(*(t.detach().requires_grad_(True) for t in tensors))
+            for o in out if isinstance(out, tuple) else [out]:
+                assert o.requires_grad
+        ops = torch.ops.gwb200
+        (_, norm), (_, qk), (_, gated), _ = _fake_calls()
+        y, mean, rstd = ops.layer_norm_stats(*norm, 1e-6)
+        h, kept = ops.gated_linear_keep(*gated, 0)
+        assert mean.shape == rstd.shape == (10,) and mean.dtype == torch.float32
+        for mask in ([True] * 5, [True, False, True, False, True]):
+            for given, grads in ((norm, ops.layer_norm_backward(y, norm[0], mean, rstd, *norm[1:], mask)),
+                                 (gated, ops.gated_linear_backward(h, *gated, kept, 0, mask)),
+                                 (gated, ops.gated_linear_backward(h, *gated, None, 0, mask))):
+                for t, g, on in zip(given, grads, mask):
+                    assert g.shape == (t.shape if on else (0,)) and g.dtype == t.dtype
+
+
+@pytest.mark.gpu
+def test_fake_tensors_trace_gradients(cuda_ready):
+    """Forward and backward shapes of every operator through autograd."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        for call, tensors in _fake_calls():
+            for some in (tensors, tensors[:1]):
+                leaves = [t.detach().requires_grad_(any(t is s for s in some)) for t in tensors]
+                out = call(*leaves)
+                out = list(out) if isinstance(out, tuple) else [out]
+                wanted = [t for t in leaves if t.requires_grad]
+                grads = torch.autograd.grad(out, wanted, [torch.ones_like(o) for o in out],
+                                            allow_unused=True)
+                assert grads[0] is not None
+                for t, g in zip(wanted, grads):
+                    assert g is None or (g.shape == t.shape and g.dtype == t.dtype)
+
+
 def _dual_calls(calls):
     """Calls with a tangent on one of their tensors, by forward_ad and by jvp."""
     from torch.autograd import forward_ad
@@ -388,3 +431,48 @@ def test_forward_mode_is_refused_on_the_gpu(cuda_ready):
     for dual in _dual_calls(calls):
         with pytest.raises(SvdqB200Error, match="forward-mode"):
             dual()
+
+
+@pytest.mark.gpu
+def test_compiled_training_step(cuda_ready):
+    """A step through torch.compile gives the eager bits, forward and backward."""
+    import gen_worker_b200 as gw
+
+    torch.manual_seed(1)
+    ff = gw.GatedFeedForward(64, 72, bias=True, device="cuda")
+    norm = gw.ModulatedLayerNorm(64, device="cuda")
+    rope = gw.RotaryEmbedding(16, device="cuda")
+    pos = torch.arange(40, device="cuda")
+
+    def step(x, s, t):
+        a, _ = rope(norm(x, s, t).view(2, 40, 4, 16), None, pos)
+        return ff(a.reshape(2, 40, 64))
+
+    leaves = [torch.randn(*n, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+              for n in ((2, 40, 64), (2, 64), (2, 64))]
+    want = step(*leaves)
+    dh = torch.randn_like(want)
+    params = [*leaves, *ff.parameters(), *norm.parameters()]
+    grads = torch.autograd.grad(want, params, dh)
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(*leaves)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, params, dh), grads):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_saved_tensor_hooks(cuda_ready):
+    """Kept tensors pass through saved-tensor hooks (offload to the host)."""
+    import gen_worker_b200 as gw
+
+    x = torch.randn(40, 64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    w = torch.randn(72, 64, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+
+    def step():
+        h = gw.gated_linear(gw.layer_norm(x), w, w)
+        return torch.autograd.grad(h, [x, w], torch.ones_like(h))
+
+    want = step()
+    with torch.autograd.graph.save_on_cpu():
+        got = step()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
