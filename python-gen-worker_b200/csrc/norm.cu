@@ -1010,21 +1010,31 @@ __global__ void __launch_bounds__(512) sums_kernel(const SumArgs a) {
   if (weights && blockIdx.y == gridDim.y - 1) {
     const uint32_t total = (uint32_t)(a.samples * a.chunks);   // at most 2^31
     float dw = 0.0f, db = 0.0f;
-    if (c < a.D)
+    const auto add = [&](auto scaled) {
       for (uint32_t i0 = w; i0 < total; i0 += WARPS * RUN) {
         const uint32_t end = min(total, i0 + WARPS * RUN);
         float rw = 0.0f, rb = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t i = i0; i < end; i += WARPS) {
           const float* p = a.partial + i * 2 * (int64_t)a.D + c;
-          float s[1], up = 1.0f;
-          if (a.s.p) { load_param<T, 1>(a.s, i / (uint32_t)a.chunks, c, s); up += s[0]; }
-          rb += up * __ldg(p);
-          rw += up * __ldg(p + a.D);
+          if constexpr (decltype(scaled)::value) {
+            float s[1];
+            load_param<T, 1>(a.s, i / (uint32_t)a.chunks, c, s);
+            rb = fmaf(1.0f + s[0], __ldg(p), rb);
+            rw = fmaf(1.0f + s[0], __ldg(p + a.D), rw);
+          } else {
+            rb += __ldg(p);
+            rw += __ldg(p + a.D);
+          }
         }
         dw += rw;
         db += rb;
       }
+    };
+    if (c < a.D) {
+      if (a.s.p) add(std::true_type{});
+      else add(std::false_type{});
+    }
     join(dw, db);
     if (w == 0 && c < a.D) {
       const auto put = [&](void* o, float v) {
