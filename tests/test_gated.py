@@ -269,6 +269,37 @@ def test_negative_tail_is_relative(cuda_ready, m, act, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 150])
+def test_erf_gelu_over_its_whole_range(cuda_ready, m):
+    """Gates in [-12, 12]: act(g) = g times the normal distribution function,
+    down to 1e-32 in bfloat16. The argument of exp, at most 72, is off by 2 U
+    and exp itself by 2 + 1.16 * 72 ulp: 144 + 172 U; what exp multiplies and
+    the products add under 30 U: 350 U of the value."""
+    f = 1536
+    g = torch.linspace(-12.0, 12.0, f).bfloat16()
+    p = make(m, 8, f, torch.bfloat16)
+    p = {"x": torch.zeros_like(p["x"]), "w_gate": torch.zeros_like(p["w_gate"]),
+         "w_up": torch.zeros_like(p["w_up"])}
+    p["x"][0, 0], p["w_gate"][:, 0], p["w_up"][:, 0] = 1.0, g, 1.0
+    from gen_worker_b200 import gated_linear
+
+    h = gated_linear(*(t.cuda() for t in p.values()), activation="gelu")[0].double().cpu()
+    # erfc: torch's ndtr cancels in its own tail (0 at -12, where it is 1.8e-33)
+    want = g.double() * 0.5 * torch.special.erfc(g.double() * -0.5 ** 0.5)
+    assert ((h - want).abs() <= want.abs() * (half_step(torch.bfloat16) + 350 * U)).all()
+    bad = torch.tensor([float("inf"), float("-inf"), float("nan"), 3e38, -3e38]).bfloat16()
+    w = torch.zeros(8, 8, dtype=torch.bfloat16)
+    w[:5, 0] = bad
+    one = torch.zeros(1, 8, dtype=torch.bfloat16)
+    one[0, 0] = 1.0
+    up = torch.zeros(8, 8, dtype=torch.bfloat16)
+    up[:, 0] = 1.0
+    h = gated_linear(one.cuda(), w.cuda(), up.cuda(), activation="gelu")[0].float().cpu()
+    assert torch.isinf(h[0]) and torch.isnan(h[1]) and torch.isnan(h[2])
+    assert h[3] == bad[3].float() and h[4] == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("recompute", [False, True])
 def test_infinite_neighbour_of_finite_gradients(cuda_ready, recompute):
     """One infinite column of a group of 64: the other columns' gradients stay
