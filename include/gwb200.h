@@ -365,7 +365,7 @@ int gwb_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64
 /* Gated feed-forward projections, bf16 or f16 (`dtype` GWB_DTYPE_BF16 /
  * _F16): h [M, F] = act(x w_gate^T + b_gate) * (x w_up^T + b_up), one kernel.
  * x [M, D] (row stride x_stride), w_gate / w_up [F, D] contiguous, biases [F]
- * or NULL; `activation` GWB_ACT_*. f32 accumulation, one rounding. D % 8 == 0,
+ * or NULL; `activation` GWB_ACT_*. f32 accumulation, h rounded once. D % 8 == 0,
  * F % 8 == 0, strides % 8 == 0, 16-byte aligned pointers. M == 0 is a no-op. */
 enum { GWB_ACT_SILU = 0, GWB_ACT_GELU = 1, GWB_ACT_GELU_TANH = 2 };
 
@@ -390,7 +390,8 @@ int64_t gwb_gated_linear_backward_work(int64_t M, int64_t D, int64_t F);
  * dw_gate / dw_up [F, D], db_gate / db_up [F], from dh [M, F] (row stride
  * dh_stride). `kept` from gwb_gated_linear_keep on the same arguments, or NULL:
  * the projections are then computed again. dg and du are rounded to `dtype`
- * as the operands of the gradients' products. No atomics: the same call gives
+ * as the operands of the gradients' products; the bias gradients add them in
+ * f32 before that. No atomics: the same call gives
  * the same bits. */
 int gwb_gated_linear_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
                               const void* w_gate, const void* w_up, const void* b_gate,

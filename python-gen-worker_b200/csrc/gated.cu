@@ -114,9 +114,9 @@ struct ActValue { float act, slope; };
 // P is the minimax polynomial of that for z up to 13.5, where the tail leaves
 // f32's range, by Lawson's iteration in 64 bits: 1.3e-7 of the value. (1 + erf
 // would cancel: off by 4 % at -5, by all of it from -5.6 on. erfcf holds, but
-// cannot share the slope's exponential and is longer: forward 4608 x 3072 ->
-// 12288, which the tensor pipe should bound, took 610 to 670 us with it and
-// takes 505.)
+// cannot share the slope's exponential and is longer: run in turn with the erf
+// form, forward calls of 4608 x 3072 -> 12288 and 1531 x 1416 -> 3880 took 9 to
+// 15 % more with it; this form takes what the erf form does.)
 __device__ __forceinline__ float normal_tail(float z, float e) {
   const float t = __fdividef(1.0f, fmaf(0.3f, z, 1.0f));
   float p = 0.03593185171484947f;

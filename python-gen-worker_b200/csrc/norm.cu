@@ -178,7 +178,7 @@ struct FwdPlan {
 // A warp takes whole rows (32 / L at a time, L lanes each), E elements a
 // lane, from its own ring of bulk copies: no barrier but the one that shares
 // g and h, and few instructions a row besides the arithmetic (18432 x 3072
-// bf16 with scale and shift: 45 us, 5.0 TB/s; without parameters 33, 6.8 TB/s:
+// bf16 with scale and shift: 46 us, 4.9 TB/s; without parameters 33, 6.8 TB/s:
 // the rest is g and h coming out of shared memory for every row). VECTOR: rows and parameters lie on 16 bytes, a lane has vectors
 // lane, lane + L, ...; else elements lane, lane + L, ..., so that any
 // alignment reads shared memory without conflicts.

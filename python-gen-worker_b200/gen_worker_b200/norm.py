@@ -27,7 +27,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     """x [..., D] (float32, bfloat16 or float16) -> y of x's shape and type,
     contiguous. ``weight`` / ``bias`` [D]; ``scale`` / ``shift`` [D], [B, D] or
     [B, 1, ..., 1, D] with B = 1 or x's first size. Each may be absent; each
-    pair is float32 or of x's type. Differentiable once in all of them.
+    pair is float32 or of x's type. Differentiable once in all of them, in
+    reverse mode (``create_graph=True`` is refused).
 
     Rows of x may lie at any one stride (a slice of a wider tensor); an x
     whose rows do not is copied first. Work is enqueued on the current stream

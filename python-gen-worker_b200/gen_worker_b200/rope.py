@@ -74,7 +74,9 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, axes: Sequence
       frequency is divided by ``factor`` and the highest kept;
     * ``by_parts``: pairs that turn more than ``fast_turns`` times over
       ``trained_length`` are kept, pairs under ``slow_turns`` divided by
-      ``factor``, a linear ramp between; attention scale 0.1 ln(factor) + 1.
+      ``factor``, a linear ramp between over the number of turns; attention
+      scale 0.1 ln(factor) + 1. (Some code ramps over the pair's index between
+      rounded bounds instead: frequencies of such a checkpoint are other ones.)
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise SvdqB200Error(f"rotary_dim {rotary_dim} is not a positive even number")
