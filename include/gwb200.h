@@ -313,7 +313,9 @@ int gwb_awq_w4a16_mm(const void* x, const void* weight, const void* wscales, con
 /* ---- Transformer-block operators beside the quantised linears: layer norm
  * with modulation, rotary positions, gated feed-forward projections. No counterpart in the reference's own
  * code, which leaves them to its model library. `dtype` codes:
- * GWB_DTYPE_F32 / _BF16 / _F16. Strides are in elements; pointers and strides
+ * GWB_DTYPE_F32 / _BF16 / _F16. Rows and features number 2^30 at most (2097120
+ * features where a norm's parameter gradients are asked for); more is
+ * GWB_E_CAPACITY. Strides are in elements; pointers and strides
  * need only the element's alignment (16-byte ones run faster). */
 enum { GWB_DTYPE_F32 = 0, GWB_DTYPE_BF16 = 1, GWB_DTYPE_F16 = 2 };
 

@@ -65,6 +65,9 @@ inline int check_w4a4_shape(int64_t M, int64_t N, int64_t K, int rank_pad) {
   return GWB_SUCCESS;
 }
 
+// The block operators round sizes up and step by tiles in 32 bits.
+inline bool over_capacity(int64_t n) { return n > (1 << 30); }
+
 inline bool known_dtype(int d) { return d == GWB_F32 || d == GWB_BF16 || d == GWB_F16; }
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -404,6 +407,7 @@ int gwb_layer_norm(const void* x, int64_t x_stride, const void* weight, const vo
   if (M == 0) return GWB_SUCCESS;
   if (!fits_int(M) || !fits_int(D) || D == 0 || rows_per_mod <= 0 || M % rows_per_mod)
     return GWB_E_SHAPE;
+  if (over_capacity(M) || over_capacity(D)) return GWB_E_CAPACITY;
   if (!known_dtype(dtype) || !x || !y || (mean == nullptr) != (rstd == nullptr))
     return GWB_E_SHAPE;
   gwb::norm::FwdArgs a{x, x_stride, {weight, affine_f32 != 0, 0}, {bias, affine_f32 != 0, 0},
@@ -426,7 +430,10 @@ int gwb_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, in
                             void* dscale, void* dshift, float* work, void* stream) {
   if (!fits_int(M) || !fits_int(D) || D == 0 || rows_per_mod < 0 || !known_dtype(dtype))
     return GWB_E_SHAPE;
+  if (over_capacity(M) || over_capacity(D)) return GWB_E_CAPACITY;
   const bool sums = dweight || dbias || dscale || dshift;
+  // tiles of 32 columns are a grid's y dimension
+  if (sums && (D + 31) / 32 > 65535) return GWB_E_CAPACITY;
   if (M == 0) {
     // no rows: the parameters' gradients are zero
     const size_t wide = affine_f32 || dtype == GWB_F32 ? 4 : 2;
@@ -460,7 +467,8 @@ int gwb_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64
                void* stream) {
   if (B < 0 || S_ < 0 || q_heads < 0 || k_heads < 0) return GWB_E_SHAPE;
   if (B == 0 || S_ == 0 || q_heads + k_heads == 0) return GWB_SUCCESS;
-  if (!fits_int(B * S_) || !fits_int(S_) || !fits_int(B) || q_heads + k_heads > (1 << 20))
+  if (!fits_int(S_) || !fits_int(B) || !fits_int(B * S_) || q_heads > (1 << 20) ||
+      k_heads > (1 << 20) || q_heads + k_heads > (1 << 20))
     return GWB_E_SHAPE;
   if (n < 0 || head_dim < 1 || head_dim > 4096 || 2 * n > head_dim || axes < 1 || axes > 64 ||
       position_kind < 0 || position_kind > 2 || !known_dtype(dtype))
@@ -486,7 +494,7 @@ static int gated_sizes(int64_t M, int64_t D, int64_t F, int activation, int dtyp
   if (!fits_int(M) || !fits_int(D) || !fits_int(F) || D == 0 || F == 0 || D % 8 || F % 8)
     return GWB_E_SHAPE;
   // tile counts are 32-bit
-  if ((M / 128 + 1) * (F / 128 + 1) > 0x7fffffff || (F / 64 + 2) * (D / 256 + 1) > 0x7ffffff ||
+  if (over_capacity(M) || over_capacity(D) || over_capacity(F) || (M / 128 + 1) * (F / 128 + 1) > 0x7fffffff || (F / 64 + 2) * (D / 256 + 1) > 0x7ffffff ||
       (M / 256 + 1) * (D / 256 + 1) > 0x7ffffff)
     return GWB_E_CAPACITY;
   if (activation < GWB_ACT_SILU || activation > GWB_ACT_GELU_TANH) return GWB_E_SHAPE;

@@ -476,3 +476,36 @@ def test_saved_tensor_hooks(cuda_ready):
     with torch.autograd.graph.save_on_cpu():
         got = step()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_sizes_past_32_bit_steps_are_refused():
+    """Sizes near 2^31, whose rounding up would wrap, and more columns than a
+    grid takes: status codes of the C entries on null pointers, nothing is
+    launched."""
+    from gen_worker_b200 import native
+
+    lib, full, capacity = native.lib(), (1 << 31) - 8, 8
+
+    def norm(m, d):
+        return lib.gwb_layer_norm(None, d, None, None, 0, None, 0, None, 0, 0, m, d, m, 1e-6, 1,
+                                  None, None, None, None)
+
+    def norm_backward(m, d, dw=None):
+        return lib.gwb_layer_norm_backward(None, d, None, d, None, None, None, None, 0, None, 0, 0, m,
+                                           d, m, 1, None, dw, None, None, None, None, None)
+
+    def gated(m, d, f):
+        a = lib.gwb_gated_linear(None, d, None, None, None, None, m, d, f, 0, 1, None, None)
+        b = lib.gwb_gated_linear_backward(None, f, None, d, *[None] * 5, m, d, f, 0, 1, *[None] * 7)
+        assert a == b
+        return a
+
+    for m, d in ((1, full), (full, 8), (1, (1 << 30) + 1)):
+        assert norm(m, d) == capacity and norm_backward(m, d) == capacity
+    assert norm(1, 1 << 30) == 1 and norm_backward(1, 1 << 30) == 1        # null pointers
+    assert norm_backward(1, 2097121, dw=16) == capacity and norm_backward(1, 2097120, dw=16) == 1
+    for sizes in ((1, 8, full), (1, full, 8), (full, 8, 8)):
+        assert gated(*sizes) == capacity
+    assert gated(1, 8, 1 << 27) == 1
+    assert lib.gwb_rotary(None, None, None, None, 1 << 62, None, None, None, None, 1 << 62, None, 0, None,
+                          None, None, 1, 1, 1, 2, 8, 1.0, 0, 0, 1, None) == 1
