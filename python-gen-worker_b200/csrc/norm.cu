@@ -1160,7 +1160,7 @@ int forward_v(const FwdArgs& a, cudaStream_t st) {
 
 // A CTA a row rather than a warp a row: up to 56 rows a multiprocessor, and for
 // wide f32 rows, whose copies leave the other form too few warps (18432 x 3072
-// f32: 86 us against 99; bf16: 60 against 50).
+// f32: 86 us a call against 99; bf16: 60 against 50).
 inline bool pairs_fit(const FwdArgs& a, int V) {
   if (a.D / V <= 32 || a.D > 4096) return false;
   return (V == 4 && a.D > 2048) || a.M <= (int64_t)sm_count() * 56;

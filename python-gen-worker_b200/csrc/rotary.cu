@@ -81,8 +81,8 @@ __device__ __forceinline__ float second_of(float p, float r, float c, float s) {
 // consecutive units (token, group of heads, item), so sizes that divide by
 // nothing leave no thread idle; its loads are in flight while it works out
 // the angles. (An item and head a thread spent more
-// instructions on indices than on the rotation: 41 us against 21 at 4608
-// tokens of 48 interleaved bf16 heads of 128, 5.3 TB/s.)
+// instructions on indices than on the rotation: 41 us against 22 at 4608
+// tokens of 48 interleaved bf16 heads of 128, 5.0 TB/s.)
 constexpr int THREADS = 256;
 // heads a thread: 32 registers of loads in flight, or eight elements
 template <int VEC, bool INTERLEAVED> constexpr int heads_of() {
